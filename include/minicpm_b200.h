@@ -84,6 +84,11 @@ extern "C" {
 #define B200_DEVERR_SLOT_RANGE 2u   /* slot_mapping entry >= num_blocks*bs      */
 #define B200_DEVERR_POS_RANGE 3u    /* position outside the cos/sin table        */
 #define B200_DEVERR_DECODE_QLEN 4u  /* max_seqlen_q = 1 but a sequence has more query tokens */
+#define B200_DEVERR_SEQ_ROW 5u      /* a table row out of range, named twice, in use, or with a bad length */
+#define B200_DEVERR_NO_PAGE 6u      /* no free page was left                     */
+#define B200_DEVERR_PAGE_RANGE 7u   /* a page id out of range, a missing page, or a release of a free page */
+#define B200_DEVERR_PAGE_SHARED 8u  /* a row would be written into a page that other sequences share */
+#define B200_DEVERR_ACCEPT 9u       /* an accepted path that does not rise, or a bad count */
 
 /*
  * Paged causal varlen attention (prefill / chunked prefill), GQA, Split-KV.
@@ -347,6 +352,185 @@ typedef struct B200KvDequantParams {
 } B200KvDequantParams;
 
 B200_API int b200_kv_dequant_pages(const B200KvDequantParams* params, void* stream);
+
+/*
+ * The attention operators below and the page operators have no counterpart in
+ * the reference.  Device-side lengths, indices and page ids that disagree with
+ * the sizes given here never lead outside the caller's buffers.
+ */
+
+/* Workspace bytes of b200_prompt_attn_fwd and b200_tree_attn_fwd for these sizes. */
+B200_API size_t b200_varlen_attn_workspace_bytes(int32_t total_q, int32_t num_seqs, int32_t num_q_heads,
+                                                 int32_t num_kv_heads, int32_t head_dim, int32_t max_seqlen_k);
+
+/*
+ * Attention of packed sequences over plain K/V rows (no cache), GQA: query row i
+ * of sequence b (rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1]) sees its keys j
+ * (rows cu_seqlens_k[b] + j) with j <= Lk - Lq + i (causal), or all Lk of them;
+ * a row that sees no key is 0.  Rows of out outside every sequence are left as
+ * they were.
+ * q, out [total_q, num_q_heads, head_dim]; k, v [total_k, num_kv_heads, head_dim];
+ * d contiguous, other strides multiples of 8 elements, pointers 16-byte aligned.
+ * F16 / BF16, head_dim 64, 128 or 256, up to 128 query heads per KV head.
+ * softmax_scale must be positive and finite.  max_seqlen_k bounds the longest
+ * sequence and only decides how far the keys may be split.
+ * Keys and values that some row of the tile sees must be finite; rows of k and v
+ * outside every sequence may hold anything.
+ * workspace: device buffer of b200_varlen_attn_workspace_bytes(...), 16-byte
+ * aligned, not shared by calls that overlap.
+ */
+typedef struct B200PromptAttnParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const void* cu_seqlens_q; /* [num_seqs + 1] */
+  const void* cu_seqlens_k; /* [num_seqs + 1]; may be cu_seqlens_q */
+  int64_t q_stride_t, q_stride_h;
+  int64_t k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h;
+  int64_t out_stride_t, out_stride_h;
+  int32_t seqlen_dtype; /* I32 / I64 */
+  int32_t dtype;
+  int32_t num_seqs;
+  int32_t total_q;
+  int32_t total_k;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t max_seqlen_k;
+  int32_t causal;
+  float softmax_scale;
+  void* workspace;
+  size_t workspace_bytes;
+} B200PromptAttnParams;
+
+B200_API int b200_prompt_attn_fwd(const B200PromptAttnParams* params, void* stream);
+
+/*
+ * Attention of drafted token trees over a paged cache (speculative decoding).
+ * The last n = cu_seqlens_q[b + 1] - cu_seqlens_q[b] keys of sequence b are its
+ * drafted tokens (their K/V rows are in the cache already); query row i sees the
+ * context, keys [0, seqused_k[b] - n), and drafted key j iff
+ * tree_mask[cu_seqlens_q[b] + i, j] is nonzero (columns at or past mask_cols are
+ * not seen).  A row that sees no key is 0.  tree_mask: one byte per entry,
+ * [total_q, mask_cols], row stride mask_stride.  Everything else as in
+ * b200_paged_attn_fwd (the cache layout and its limits) and
+ * b200_prompt_attn_fwd (scale, workspace, finiteness).
+ */
+typedef struct B200TreeAttnParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const void* tree_mask;
+  const void* block_table;
+  const void* cu_seqlens_q;
+  const void* seqused_k;
+  int64_t q_stride_t, q_stride_h;
+  int64_t k_stride_block, k_stride_tok, k_stride_head;
+  int64_t v_stride_block, v_stride_tok, v_stride_head;
+  int64_t out_stride_t, out_stride_h;
+  int64_t mask_stride;
+  int64_t block_table_stride;
+  int32_t mask_cols;
+  int32_t block_table_cols;
+  int32_t block_table_dtype; /* I32 / I64 */
+  int32_t seqlen_dtype;      /* I32 / I64 */
+  int32_t dtype;
+  int32_t num_seqs;
+  int32_t total_q;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t block_size;
+  int32_t num_blocks;
+  int32_t max_seqlen_k;
+  float softmax_scale;
+  void* workspace;
+  size_t workspace_bytes;
+} B200TreeAttnParams;
+
+B200_API int b200_tree_attn_fwd(const B200TreeAttnParams* params, void* stream);
+
+/*
+ * The caches that a page operator works on: the K and V tensors of every layer,
+ * [num_blocks, block_size, num_kv_heads, row], of any element type (bytes are
+ * moved as they are; rows may carry their scale inline).  All share the shape and
+ * the strides (bytes); a page is one dense run, tokens or heads outermost.
+ * Pointers, strides and rows are multiples of 4 bytes.  The caches are distinct.
+ */
+typedef struct B200PageCaches {
+  const void* const* base; /* host array of num_caches device pointers, 1 .. 256 */
+  int32_t num_caches;
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int64_t row_bytes;
+  int64_t stride_block, stride_tok, stride_head;
+} B200PageCaches;
+
+/* Block table, lengths and page reference counts of a pool of sequences. */
+typedef struct B200SeqTable {
+  void* block_table;   /* [max_seqs, cols], row stride in elements, -1 = no page */
+  void* seq_lens;      /* [max_seqs] tokens */
+  int32_t* ref_counts; /* [num_blocks], 0 = free */
+  int64_t stride;
+  int32_t cols;
+  int32_t max_seqs;
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t table_dtype;  /* I32 / I64 */
+  int32_t seqlen_dtype; /* I32 / I64 */
+} B200SeqTable;
+
+/*
+ * Page src_pages[i] -> page dst_pages[i] in every cache, i < num_pairs.  A pair
+ * with a negative index is skipped (padding); an index past the cache is skipped
+ * and recorded (B200_DEVERR_PAGE_RANGE).  A destination may be neither named
+ * twice nor a source of another pair: the copies run at the same time.
+ */
+B200_API int b200_copy_pages(const B200PageCaches* caches, const void* src_pages, const void* dst_pages,
+                             int32_t num_pairs, int32_t index_dtype, void* stream);
+
+/*
+ * Row children[i] of the table becomes a copy of row parents[i]: full pages are
+ * shared (their counts rise by one), the used rows of a partial last page go to a
+ * free page of the child's own -- the lowest free ones, in the order of the
+ * entries -- and seq_lens[child] = seq_lens[parent].  A child's row must be empty
+ * (length 0) and is named once.  Entries with a negative index are padding.  An
+ * entry that cannot be served (a row out of range, in use or named before:
+ * B200_DEVERR_SEQ_ROW; no page left: B200_DEVERR_NO_PAGE; a table that names no
+ * page: B200_DEVERR_PAGE_RANGE) is recorded and leaves its child empty.
+ * workspace: b200_fork_workspace_bytes(num_entries, max_seqs), 16-byte aligned.
+ */
+B200_API size_t b200_fork_workspace_bytes(int32_t num_entries, int32_t max_seqs);
+B200_API int b200_fork_sequences(const B200PageCaches* caches, const B200SeqTable* table, const void* parents,
+                                 const void* children, int32_t num_entries, int32_t index_dtype, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/*
+ * Empties the rows named: every page's count falls by one, the row's entries
+ * become -1 and its length 0.  A page whose count reaches 0 is free.  Naming a row
+ * twice, or an empty one, releases nothing twice; negative rows are padding.
+ */
+B200_API int b200_free_sequences(const B200SeqTable* table, const void* rows, int32_t num_rows, int32_t index_dtype,
+                                 void* stream);
+
+/*
+ * After the verification of drafts: for sequence b and i < num_accepted[b], the
+ * K/V row at position context_lens[b] + accepted[b, i] moves to context_lens[b] +
+ * i in every cache, and seq_lens[b] = context_lens[b] + num_accepted[b].
+ * accepted[b, :num_accepted[b]] rises strictly (an ancestor path of a tree whose
+ * parents come first).  With ref_counts, the pages behind the new length are
+ * released, and a row is not written into a page that is shared.  A path is cut
+ * before its first entry that does not rise (B200_DEVERR_ACCEPT), has no page
+ * (B200_DEVERR_PAGE_RANGE) or would write a shared page (B200_DEVERR_PAGE_SHARED).
+ * seq_lens is written for every row of the table and is not context_lens.
+ */
+B200_API int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable* table, const void* context_lens,
+                                const void* accepted, int64_t accepted_stride, int32_t most, const void* num_accepted,
+                                int32_t index_dtype, void* stream);
 
 /* Message of the last failed call on this host thread ("" if none). */
 B200_API const char* b200_last_error(void);

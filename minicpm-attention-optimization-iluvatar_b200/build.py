@@ -2,9 +2,9 @@
 
     python build.py            # from this directory, or call build() from Python
 
-One nvcc invocation over ``csrc/b200_lib.cu`` (the kernels are headers it
-includes), for ``-gencode arch=compute_100a,code=sm_100a`` only, with the
-CUDA runtime linked statically so the library does not depend on which
+One nvcc invocation per ``csrc/*.cu`` (the kernels are headers they include),
+all at once, for ``-gencode arch=compute_100a,code=sm_100a`` only, then one
+link with the CUDA runtime static so the library does not depend on which
 libcudart the host process loaded first.
 """
 
@@ -14,19 +14,18 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 REPO = HERE.parent
-SRC = HERE / "csrc" / "b200_lib.cu"
 OUT = HERE / "minicpm_b200" / "_lib" / "libminicpm_b200.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
+    "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     "--expt-relaxed-constexpr",
-    "-cudart", "static",
 ]
 
 
@@ -38,7 +37,7 @@ def nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted((HERE / "csrc").glob("*.cu*")) + [REPO / "include" / "minicpm_b200.h"]
+    return sorted((HERE / "csrc").glob("*.cu*")) + sorted((HERE / "csrc").glob("*.h")) + [REPO / "include" / "minicpm_b200.h"]
 
 
 def up_to_date() -> bool:
@@ -53,15 +52,29 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         return OUT
     OUT.parent.mkdir(parents=True, exist_ok=True)
     tmp = OUT.with_suffix(".so.tmp")
-    cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", str(REPO / "include"), "-I", str(HERE / "csrc"),
-           str(SRC), "-o", str(tmp)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    if verbose and (res.stdout or res.stderr):
-        print(res.stdout + res.stderr, flush=True)
+    inc = ["-I", str(REPO / "include"), "-I", str(HERE / "csrc")]
+
+    def run(cmd: list[str]) -> str:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{' '.join(cmd)} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        return res.stdout + res.stderr
+
+    def compile_one(src: Path) -> tuple[Path, str]:
+        obj = OUT.parent / (src.stem + ".o")
+        if not force and obj.exists() and all(p.stat().st_mtime <= obj.stat().st_mtime for p in headers + [src]):
+            return obj, ""
+        return obj, run([nvcc(), *NVCC_FLAGS, *(extra or []), *inc, "-c", str(src), "-o", str(obj)])
+
+    headers = [p for p in sources() if p.suffix != ".cu"] + [Path(__file__)]
+    units = [p for p in sources() if p.suffix == ".cu"]
+    with ThreadPoolExecutor(max_workers=len(units)) as pool:
+        done = list(pool.map(compile_one, units))
+    log = "".join(text for _, text in done)
+    log += run([nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-cudart", "static",
+                *(str(obj) for obj, _ in done), "-o", str(tmp)])
+    if verbose and log:
+        print(log, flush=True)
     os.replace(tmp, OUT)
     return OUT
 

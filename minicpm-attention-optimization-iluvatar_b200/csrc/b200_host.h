@@ -1,0 +1,33 @@
+// b200_host.h -- host helpers that the translation units of the library share
+// (defined in b200_lib.cu unless inline here).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace b200_host {
+
+constexpr int kNumSmsB200 = 148;
+
+// Sets the calling thread's error message and returns `code`.
+int fail(int code, const char* fmt, ...);
+const char* last_error();
+// The launch error of the last kernel, as a status.
+int check_launch(const char* what);
+// SMs of the current device (148 without one).
+int sm_count();
+// A tensor map with 128-byte swizzle, 256-byte L2 promotion and zero fill.
+int encode_map(CUtensorMap* map, CUtensorMapDataType dt, cuuint32_t rank, const void* base, const cuuint64_t* dims,
+               const cuuint64_t* strides_bytes, const cuuint32_t* box, const char* what);
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+// The device error word of each translation unit besides b200_lib.cu: read and cleared.
+cudaError_t prompt_device_error(unsigned int* code);
+cudaError_t tree_device_error(unsigned int* code);
+cudaError_t pages_device_error(unsigned int* code);
+
+}  // namespace b200_host

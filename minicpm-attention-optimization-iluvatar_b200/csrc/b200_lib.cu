@@ -1,6 +1,8 @@
 // b200_lib.cu -- the C ABI declared in include/minicpm_b200.h.
 //
-// One translation unit: the kernels live in the headers included below.
+// The kernels live in the headers included below; prompt and draft-tree
+// attention and the cache's page operators have translation units of their own
+// (b200_prompt.cu, b200_tree.cu, b200_pages.cu), which compile in parallel.
 // Host code validates arguments (mirroring the reference's ValueError checks
 // in kernels/triton_split_kv_paged.py:249-281 and
 // kernels/triton_rope_kv_cache.py:219-260 where they apply to raw pointers),
@@ -20,6 +22,7 @@
 #include <mutex>
 
 #include "minicpm_b200.h"
+#include "b200_host.h"
 #include "paged_attention.cuh"
 #include "paged_decode.cuh"
 #include "rope_kv_cache.cuh"
@@ -47,9 +50,13 @@ __global__ void __launch_bounds__(32, 1) wait_selftest_kernel() {
 
 }  // namespace b200
 
-namespace {
+namespace b200_host {
 
+namespace {
 thread_local char g_last_error[512] = "";
+}  // namespace
+
+const char* last_error() { return g_last_error; }
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -65,10 +72,6 @@ int check_launch(const char* what) {
   return B200_OK;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-constexpr int kNumSmsB200 = 148;
-
 int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return kNumSmsB200;
@@ -76,7 +79,7 @@ int sm_count() {
   return n;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -94,14 +97,26 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType dt, cuuint32_t rank, const 
   auto enc = tensor_map_encoder();
   if (!enc) return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
   cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
-  const CUresult r = enc(map, dt, rank, const_cast<void*>(base), dims, strides_bytes, box, elem_strides,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return enc(map, dt, rank, const_cast<void*>(base), dims, strides_bytes, box, elem_strides,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int dev = 0;
+  // A host thread's first CUDA work may be this driver call, before any runtime
+  // call has made the device's primary context current in the thread.
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = encode();
   if (r != CUDA_SUCCESS) return fail(B200_ERR_INVALID, "tensor map for %s rejected by the driver (CUresult %d)", what, (int)r);
   return B200_OK;
 }
 
-size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+}  // namespace b200_host
+
+namespace {
+
+using namespace b200_host;
 
 // Prefill workspace: the schedule's counters and per-sequence / per-query-unit
 // arrays, the work list, and (num_splits > 1) the split units' list and
@@ -325,7 +340,7 @@ extern "C" {
 
 int b200_abi_version(void) { return B200_ABI_VERSION; }
 
-const char* b200_last_error(void) { return g_last_error; }
+const char* b200_last_error(void) { return b200_host::last_error(); }
 
 int32_t b200_choose_num_splits(int32_t total_q, int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
                                int32_t max_seqlen_k) {
@@ -504,8 +519,9 @@ int b200_paged_attn_fwd(const B200AttnParams* p, void* stream) {
   sa.units = reinterpret_cast<int4*>(ws + w.units_off);
   sa.split_units = reinterpret_cast<int4*>(ws + w.split_units_off);
   sa.unit_count = reinterpret_cast<int*>(ws + w.count_off);
-  cudaFuncSetAttribute(b200::attn_schedule_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, b200::kSchedSmemBytes);
-  b200::attn_schedule_kernel<<<1, b200::kSchedThreads, b200::kSchedSmemBytes, s>>>(sa);
+  cudaFuncSetAttribute(b200::attn_schedule_kernel<b200::kFormPaged>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       b200::kSchedSmemBytes);
+  b200::attn_schedule_kernel<b200::kFormPaged><<<1, b200::kSchedThreads, b200::kSchedSmemBytes, s>>>(sa);
   if (int r = check_launch("attn_schedule_kernel")) return r;
 
   b200::AttnKernelArgs a{};
@@ -950,6 +966,12 @@ int b200_device_error(void* stream, uint32_t* code) {
   unsigned int v = 0, zero = 0;
   e = cudaMemcpyFromSymbol(&v, b200::g_device_error, sizeof(v));
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(b200::g_device_error, &zero, sizeof(zero));
+  // Each translation unit has an error word of its own; the first set one is reported, all are cleared.
+  for (auto read : {b200_host::prompt_device_error, b200_host::tree_device_error, b200_host::pages_device_error}) {
+    unsigned int u = 0;
+    if (e == cudaSuccess) e = read(&u);
+    if (v == 0) v = u;
+  }
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "device error word: %s", cudaGetErrorString(e));
   *code = v;
   return B200_OK;

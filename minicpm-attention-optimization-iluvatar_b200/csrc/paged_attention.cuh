@@ -54,6 +54,22 @@
 // P, which they do after their epilogue has read the previous unit's O_t.
 // TMEM: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512); P_t in the
 // first 64 columns of S_t.
+//
+// Forms (kForm): kFormPaged is the causal paged attention above.
+//   kFormPrompt  K and V are plain rows [total_k, KH, D] addressed through
+//                cu_seqlens_k: a tile is one 128-row TMA box per 64 columns of
+//                head_dim (2 copies where a paged tile takes 8 page slices).
+//                Causal, or bidirectional (full = 1: a row sees [0, L)).  Rows
+//                of the last tile at or past L belong to the next sequence;
+//                their V rows are zeroed like a page's tail.
+//   kFormTree    paged; the last q_len keys of a sequence are drafted tokens,
+//                row i sees the context [0, L - q_len) and drafted key j iff
+//                tree_mask[row i, j].  Only tiles that reach past the context
+//                are masked; their mask bits are gathered by ballots, one
+//                coalesced read of the mask row per query position.
+// Both keep every index inside the caller's sizes (rows, mask columns, work
+// list), whatever the device-side lengths say, and hold the partial O of split
+// units in fp32.
 // Registers: launched at 168 per thread (the 384-thread limit); the first
 // warpgroup gives back down to 104 and the softmax warpgroups take 200 each
 // (104 + 2 x 200 = 3 x 168, the launch's total).
@@ -110,9 +126,12 @@ enum : int {
 // A claimed unit as the producer publishes it: (seq, qunit, kvh, split, the
 // unit's split count, its partial-output slot), then cu_q[seq], cu_q[seq + 1],
 // seqused[seq] and a valid flag (0 ends the loop).
+// kFormPrompt also carries the first K/V row of the sequence.
 struct UnitEntry {
-  int seq, qunit, kvh, split, nsplit, slot, q_begin, q_end, seq_len, valid;
+  int seq, qunit, kvh, split, nsplit, slot, q_begin, q_end, seq_len, valid, k_begin;
 };
+
+enum : int { kFormPaged = 0, kFormPrompt = 1, kFormTree = 2 };
 
 // Work-list entry: x = sequence, y = query unit, z = KV head | split << 16 |
 // split count << 24, w = partial-output slot of a split unit (-1 unsplit).
@@ -152,6 +171,13 @@ struct AttnKernelArgs {
   int num_splits;     // the most splits any unit has (the partial buffers' split stride)
   int head_dim;       // 128, or 64 (the upper 64 columns of every tile are TMA zero fill)
   float scale_log2;   // softmax_scale * log2(e)
+  // kFormPrompt / kFormTree
+  const void* cu_k;          // kFormPrompt: [num_seqs + 1]
+  const uint8_t* tree_mask;  // kFormTree: [total_q, mask_cols], nonzero = seen
+  int64_t mask_stride;
+  int mask_cols;
+  int total_k;
+  int full;                  // every row's keys end at L (bidirectional, or masked by the tree)
 };
 
 // K/V tensor maps.  Up to kMaxHeadMaps KV heads: one 5-D map per head,
@@ -188,18 +214,44 @@ struct UnitGeom {
   int q_abs_min;
 };
 
-// KV tiles of a query unit's whole causal key range [0, min(L, last row + 1)).
-__device__ __forceinline__ int qunit_full_tiles(int q_len, int seq_len, int qunit, int pos_per_unit) {
+// Query rows [begin, end) and keys of a sequence as the bounded forms read
+// them: clipped to the caller's sizes.
+struct SeqBounds {
+  int q_begin, q_end, seq_len, k_begin;
+};
+template <int kForm, typename Args>
+__device__ __forceinline__ SeqBounds seq_bounds(const Args& a, int b) {
+  SeqBounds s{};
+  s.q_begin = load_index(a.cu_q, b, a.len_i64);
+  s.q_end = load_index(a.cu_q, b + 1, a.len_i64);
+  if (kForm != kFormPaged) {
+    s.q_begin = min(max(s.q_begin, 0), a.total_q);
+    s.q_end = min(max(s.q_end, s.q_begin), a.total_q);
+  }
+  if (kForm == kFormPrompt) {
+    s.k_begin = min(max(load_index(a.cu_k, b, a.len_i64), 0), a.total_k);
+    s.seq_len = min(max(load_index(a.cu_k, b + 1, a.len_i64), s.k_begin), a.total_k) - s.k_begin;
+  } else {
+    s.seq_len = load_index(a.seqused, b, a.len_i64);
+    // A table row holds bt_cols pages; keys past them do not exist.
+    if (kForm == kFormTree)
+      s.seq_len = static_cast<int>(min(static_cast<int64_t>(max(s.seq_len, 0)), static_cast<int64_t>(a.bt_cols) * a.block_size));
+  }
+  return s;
+}
+
+// KV tiles of a query unit's whole key range: [0, min(L, last row + 1)), or [0, L) with `full`.
+__device__ __forceinline__ int qunit_full_tiles(int q_len, int seq_len, int qunit, int pos_per_unit, int full = 0) {
   const int pos0 = qunit * pos_per_unit;
   const int rows = min(pos_per_unit, q_len - pos0);
-  const int kv_end = min(max(seq_len, 0), seq_len - q_len + pos0 + rows);
+  const int kv_end = full ? max(seq_len, 0) : min(max(seq_len, 0), seq_len - q_len + pos0 + rows);
   return kv_end > 0 ? (kv_end + kAttnTileN - 1) / kAttnTileN : 0;
 }
 
 // Split `split` of `nsplit` covers whole tiles [split * tps, (split + 1) * tps)
 // of the unit's key range, tps = ceil(full tiles / nsplit).
 __device__ __forceinline__ UnitGeom unit_geometry(int q_begin, int q_end, int seq_len, int qunit, int split,
-                                                  int nsplit, int pos_per_unit) {
+                                                  int nsplit, int pos_per_unit, int full = 0) {
   UnitGeom u;
   u.q_begin = q_begin;
   u.q_len = q_end - q_begin;
@@ -207,7 +259,7 @@ __device__ __forceinline__ UnitGeom unit_geometry(int q_begin, int q_end, int se
   u.pos0 = qunit * pos_per_unit;
   const int rows = min(pos_per_unit, u.q_len - u.pos0);
   u.q_abs_min = seq_len - u.q_len + u.pos0;
-  const int kv_end = max(min(max(seq_len, 0), u.q_abs_min + rows), 0);
+  const int kv_end = full ? max(seq_len, 0) : max(min(max(seq_len, 0), u.q_abs_min + rows), 0);
   const int n_full = (kv_end + kAttnTileN - 1) / kAttnTileN;
   const int tps = nsplit > 1 ? (n_full + nsplit - 1) / nsplit : n_full;
   u.split_begin = split * tps * kAttnTileN;
@@ -258,13 +310,14 @@ __device__ __forceinline__ void mbar_wait_drain(uint32_t bar, uint32_t parity) {
 // kNarrow: head_dim 64.  K/V tiles fill the first 16 KB of their ring slots (one
 // 64-column half per row), S = Q K^T is 4 UMMAs (K = 64) and O += P V runs with
 // N = 64 (O in the first 64 of the tile's 128 TMEM columns).
-template <typename T, bool kHeadMaps, bool kWide, bool kNarrow>
+template <typename T, bool kHeadMaps, bool kWide, bool kNarrow, int kForm = kFormPaged>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     paged_attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ KvHeadMaps maps,
                           const AttnKernelArgs a) {
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kTilesPerUnit = kWide ? 1 : kAttnTilesPerUnit;
   constexpr int kFillsPerTile = kWide ? 4 : 2;  // ring slots per KV tile: K (, K hi), V (, V hi)
+  static_assert(kForm != kFormPrompt || !kHeadMaps, "plain rows use one map for all heads");
   griddep_wait();  // launched as a programmatic dependent of the schedule kernel
 
   extern __shared__ uint8_t smem_raw[];
@@ -336,10 +389,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     e.q_end = ring[r].q_end;
     e.seq_len = ring[r].seq_len;
     e.valid = ring[r].valid;
+    e.k_begin = 0;  // only the producer reads it
     return true;
   };
   auto geometry = [&](const UnitEntry& e) {
-    return unit_geometry(e.q_begin, e.q_end, e.seq_len, e.qunit, e.split, e.nsplit, ppu);
+    return unit_geometry(e.q_begin, e.q_end, e.seq_len, e.qunit, e.split, e.nsplit, ppu,
+                         kForm == kFormPaged ? 0 : kForm == kFormTree ? 1 : a.full);
   };
 
   if (warp < 4) {
@@ -368,9 +423,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           e.qunit = un.y;
           unpack_unit(un, e.kvh, e.split, e.nsplit);
           e.slot = un.w;
-          e.q_begin = load_index(a.cu_q, e.seq, a.len_i64);
-          e.q_end = load_index(a.cu_q, e.seq + 1, a.len_i64);
-          e.seq_len = load_index(a.seqused, e.seq, a.len_i64);
+          const SeqBounds sb = seq_bounds<kForm>(a, e.seq);
+          e.q_begin = sb.q_begin;
+          e.q_end = sb.q_end;
+          e.seq_len = sb.seq_len;
+          e.k_begin = sb.k_begin;
         }
         int ok = 1;
         if (lane == 0) {
@@ -431,9 +488,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const int v = load_index(a.block_table, bt_row + lpc, a.bt_i64);
           pg = (pos < ug.kv_hi && lp < a.bt_cols) ? v : a.num_blocks;
         };
-        int pg_cur, of_cur, pg_nxt = a.num_blocks, of_nxt = 0;
-        lookup(0, pg_cur, of_cur);
-        if (n_tiles > 1) lookup(1, pg_nxt, of_nxt);
+        int pg_cur = 0, of_cur = 0, pg_nxt = a.num_blocks, of_nxt = 0;
+        if (kForm != kFormPrompt) {
+          lookup(0, pg_cur, of_cur);
+          if (n_tiles > 1) lookup(1, pg_nxt, of_nxt);
+        }
         bool stop = false;
         for (int idx = 0; idx < kFillsPerTile * n_tiles; ++idx) {
           const int j = idx / kFillsPerTile;
@@ -442,7 +501,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const int hi = kWide ? (part & 1) : 0;  // 128-column half of a head_dim-256 row
           const int slot = issued % kKvStages;
           const uint32_t ph = (issued / kKvStages) & 1;
-          if (part == 0 && j > 0) {
+          if (kForm != kFormPrompt && part == 0 && j > 0) {
             pg_cur = pg_nxt;
             of_cur = of_nxt;
             if (j + 1 < n_tiles) lookup(j + 1, pg_nxt, of_nxt);
@@ -459,7 +518,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             stop = true;
             break;
           }
-          if (kHeadMaps) {
+          if (kForm == kFormPrompt) {
+            // 128 rows x 64 columns a copy (16 KB), one per half; rows past the tensor are zero fill.
+            if (lane < (kNarrow ? 1 : 2))
+              tma_load_3d(sbase + kSmKV + slot * 32768 + lane * 16384, is_v ? &maps.v[0] : &maps.k[0],
+                          bar(BAR_KV_FULL + slot), lane * 64 + hi * 128, e.kvh, e.k_begin + ug.kv_lo + j * kAttnTileN);
+          } else if (kHeadMaps) {
             // lane c < 8 issues slice c (its own lookup): 16 keys x both halves.
             if (lane < 8) {
               const CUtensorMap* map = is_v ? &maps.v[e.kvh] : &maps.k[e.kvh];
@@ -686,12 +750,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int row_head = e.kvh * a.group + row % a.group;
       const bool row_valid = row < q_rows && row_pos < ug.q_len;
       const int q_abs = ug.q_abs_min + t * P + row / a.group;
-      const int row_hi = min(ug.split_end, q_abs + 1);
-      const int unmasked_hi = min(ug.split_end, ug.q_abs_min + t * P + 1);
+      const bool full = kForm == kFormPrompt && a.full;
+      const int row_hi = (kForm == kFormTree || full) ? ug.split_end : min(ug.split_end, q_abs + 1);
+      const int ctx = ug.seq_len - ug.q_len;  // kFormTree: keys at or past it are drafted tokens
+      const int unmasked_hi = kForm == kFormTree ? min(ug.split_end, ctx)
+                              : full             ? ug.split_end
+                                                 : min(ug.split_end, ug.q_abs_min + t * P + 1);
       // V rows [v_tail_from, v_tail_to) of the last tile: loaded page rows at or past L.
       const int last_start = ug.kv_lo + (n_tiles - 1) * kAttnTileN;
       const int v_tail_from = max(ug.seq_len - last_start, 0);
-      const int v_tail_to = min(((ug.kv_hi + kAttnSlice - 1) / kAttnSlice) * kAttnSlice - last_start, kAttnTileN);
+      const int v_tail_to = kForm == kFormPrompt
+                                ? kAttnTileN
+                                : min(((ug.kv_hi + kAttnSlice - 1) / kAttnSlice) * kAttnSlice - last_start, kAttnTileN);
 
       float m_used = -INFINITY;  // running maximum in scaled base-2 units
       float l = 0.f;
@@ -711,6 +781,30 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
         const int tile_start = ug.kv_lo + j * kAttnTileN;
         if (tile_start < ug.split_begin || tile_start + kAttnTileN > unmasked_hi) {
+          if (kForm == kFormTree) {
+            // Bit cc of word c4: key tile_start + 32 c4 + cc is seen.  The warp's
+            // rows hold few query positions; each position's bits are one
+            // coalesced read per 32 keys and a ballot.
+            uint32_t seen[4] = {0u, 0u, 0u, 0u};
+            const int first = (quarter * 32) / a.group, last = min((quarter * 32 + 31) / a.group, P - 1);
+            for (int p = first; p <= last; ++p) {
+              const bool has = tile_pos0 + p < ug.q_len;
+              const uint8_t* mrow = a.tree_mask + static_cast<int64_t>(ug.q_begin + tile_pos0 + p) * a.mask_stride;
+#pragma unroll
+              for (int c4 = 0; c4 < 4; ++c4) {
+                const int key = tile_start + c4 * 32 + lane, node = key - ctx;
+                bool see = has && key < ug.split_end;
+                if (see && node >= 0) see = node < a.mask_cols && mrow[node] != 0;
+                const uint32_t word = __ballot_sync(0xffffffffu, see);
+                if (row / a.group == p) seen[c4] = word;
+              }
+            }
+#pragma unroll
+            for (int c4 = 0; c4 < 4; ++c4)
+#pragma unroll
+              for (int cc = 0; cc < 32; ++cc)
+                if (!((seen[c4] >> cc) & 1u)) sr[c4][cc] = __float_as_uint(-INFINITY);
+          } else {
           const int lo = ug.split_begin - tile_start;
           const int hi = row_hi - tile_start;
 #pragma unroll
@@ -720,6 +814,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               const int col = c4 * 32 + cc;
               if (col < lo || col >= hi) sr[c4][cc] = __float_as_uint(-INFINITY);
             }
+          }
         }
         // Fast path: when the second half's maximum stays within the rescale
         // threshold of the running maximum, the first half's P is computed
@@ -867,12 +962,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (aborted) break;
       const float inv = 1.f / fmaxf(l, 1e-20f);
       const int tok = ug.q_begin + row_pos;
-      T* dst;
+      T* dst = nullptr;
+      float* dst32 = nullptr;  // partial O of the bounded forms
       if (e.nsplit <= 1) {
         dst = static_cast<T*>(a.out) + static_cast<int64_t>(tok) * a.out_st + static_cast<int64_t>(row_head) * a.out_sh;
       } else {
         const int64_t rowi = (static_cast<int64_t>(e.slot) * a.num_splits + e.split) * kUnitRows + t * kAttnTileM + row;
-        dst = static_cast<T*>(a.o_split) + rowi * a.head_dim;
+        if (kForm == kFormPaged) dst = static_cast<T*>(a.o_split) + rowi * a.head_dim;
+        else dst32 = static_cast<float*>(a.o_split) + rowi * a.head_dim;
         if (row_valid) {
           a.m_split[rowi] = (l > 0.f) ? m_used * 0.69314718055994530942f : -INFINITY;
           a.l_split[rowi] = l;
@@ -889,7 +986,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int cc = 0; cc < 32; ++cc) o[cc] = 0u;
         }
-        if (row_valid) {
+        if (kForm != kFormPaged && dst32) {
+          if (row_valid) {
+            float4* f4 = reinterpret_cast<float4*>(dst32 + c4 * 32);
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              f4[v] = make_float4(__uint_as_float(o[4 * v]) * inv, __uint_as_float(o[4 * v + 1]) * inv,
+                                  __uint_as_float(o[4 * v + 2]) * inv, __uint_as_float(o[4 * v + 3]) * inv);
+          }
+        } else if (row_valid) {
           uint4* d4 = reinterpret_cast<uint4*>(dst + c4 * 32);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
@@ -958,6 +1063,11 @@ struct SchedArgs {
   int uniform_splits;  // 1: every query unit is split num_splits ways
   int num_sms;
   int capacity;
+  // kFormPrompt / kFormTree: the caller's sizes, which bound what the lengths say.
+  const void* cu_k;
+  int total_q, total_k, bt_cols, block_size;
+  int max_qunits;    // room in the per-query-unit arrays
+  int full;
   int* tile_base;    // [num_seqs + 1]: query units per sequence, exclusive prefix
   int* seq_off;      // [num_seqs]: first slot of each sequence's units in the work list
   int* qunit_base;   // [query units + 1]: work units (splits x KV heads) per query unit, exclusive prefix
@@ -1092,6 +1202,7 @@ constexpr int kSchedQunitCache = 8192;
 constexpr uint32_t kSchedSmemBytes =
     16 * kSchedThreads + 4 * (kSchedBuckets + 64 + 4 * kSchedSeqCache + 1 + 4 * kSchedQunitCache + 1);
 
+template <int kForm>
 __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const SchedArgs a) {
   extern __shared__ int4 sched_smem[];
   int4* s_tail = sched_smem;                             // [kSchedThreads]
@@ -1110,10 +1221,13 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
   griddep_launch_dependents();  // the attention grid may launch; it waits for this one
 
   const bool seq_cached = a.num_seqs <= kSchedSeqCache;
+  const int full = kForm == kFormPaged ? 0 : kForm == kFormTree ? 1 : a.full;
   auto q_len = [&](int b) {
-    return seq_cached ? s_ql[b] : load_index(a.cu_q, b + 1, a.len_i64) - load_index(a.cu_q, b, a.len_i64);
+    if (seq_cached) return s_ql[b];
+    const SeqBounds sb = seq_bounds<kForm>(a, b);
+    return sb.q_end - sb.q_begin;
   };
-  auto kv_len = [&](int b) { return seq_cached ? s_L[b] : load_index(a.seqused, b, a.len_i64); };
+  auto kv_len = [&](int b) { return seq_cached ? s_L[b] : seq_bounds<kForm>(a, b).seq_len; };
 
   // 1. query units per sequence, exclusive prefix over sequences.
   int carry = 0;
@@ -1121,8 +1235,9 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
     const int b = base + threadIdx.x;
     int n = 0;
     if (b < a.num_seqs) {
-      const int ql = load_index(a.cu_q, b + 1, a.len_i64) - load_index(a.cu_q, b, a.len_i64);
-      const int L = load_index(a.seqused, b, a.len_i64);
+      const SeqBounds sb = seq_bounds<kForm>(a, b);
+      const int ql = sb.q_end - sb.q_begin;
+      const int L = sb.seq_len;
       if (seq_cached) {
         s_ql[b] = ql;
         s_L[b] = L;
@@ -1130,7 +1245,13 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
       n = ql > 0 ? (ql + a.pos_per_unit - 1) / a.pos_per_unit : 0;
     }
     int total;
-    const int before = block_exclusive_scan(n, warp_sums, total);
+    int before = block_exclusive_scan(n, warp_sums, total);
+    if (kForm != kFormPaged) {
+      // Rows that sequences share (cu_seqlens_q not rising) could name more
+      // query units than there is room for: the ones past it are dropped.
+      before = min(before, a.max_qunits - carry);
+      total = min(total, a.max_qunits - carry);
+    }
     if (b < a.num_seqs) {
       a.tile_base[b] = carry + before;
       if (seq_cached) s_tb[b] = carry + before;
@@ -1164,7 +1285,7 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
   unsigned long long my_tiles = 0;
   for (int j = j_begin, seq = seq_begin; j < j_end; ++j) {
     while (tb[seq + 1] <= j) ++seq;  // past empty sequences
-    const int n = qunit_full_tiles(q_len(seq), kv_len(seq), j - tb[seq], a.pos_per_unit);
+    const int n = qunit_full_tiles(q_len(seq), kv_len(seq), j - tb[seq], a.pos_per_unit, full);
     qs[j] = n;
     if (q_cached) s_qseq[j] = seq;
     my_tiles += static_cast<unsigned long long>(n);
@@ -1259,8 +1380,9 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
     unit = ucarry == total_units ? s_tail[threadIdx.x] : a.units[tail0 + threadIdx.x];
     int kvh, split, nsplit;
     unpack_unit(unit, kvh, split, nsplit);
-    const int q0 = seq_cached ? 0 : load_index(a.cu_q, unit.x, a.len_i64);
-    const UnitGeom g = unit_geometry(q0, q0 + q_len(unit.x), kv_len(unit.x), unit.y, split, nsplit, a.pos_per_unit);
+    const int q0 = (seq_cached || kForm != kFormPaged) ? 0 : load_index(a.cu_q, unit.x, a.len_i64);
+    const UnitGeom g =
+        unit_geometry(q0, q0 + q_len(unit.x), kv_len(unit.x), unit.y, split, nsplit, a.pos_per_unit, full);
     bucket = min(g.n_tiles, kSchedBuckets - 1);
   }
   for (int i = threadIdx.x; i < kSchedBuckets; i += kSchedThreads) hist[i] = 0;

@@ -7,6 +7,7 @@ library is missing, every operator raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -44,6 +45,11 @@ DEVERR_WAIT_TIMEOUT = 1
 DEVERR_SLOT_RANGE = 2
 DEVERR_POS_RANGE = 3
 DEVERR_DECODE_QLEN = 4
+DEVERR_SEQ_ROW = 5
+DEVERR_NO_PAGE = 6
+DEVERR_PAGE_RANGE = 7
+DEVERR_PAGE_SHARED = 8
+DEVERR_ACCEPT = 9
 
 _TORCH_DTYPES = {
     torch.float16: DTYPE_F16,
@@ -68,6 +74,14 @@ EXPORTED_SYMBOLS = (
     "b200_rope_kv_write",
     "b200_kv_cache_write",
     "b200_kv_dequant_pages",
+    "b200_varlen_attn_workspace_bytes",
+    "b200_prompt_attn_fwd",
+    "b200_tree_attn_fwd",
+    "b200_copy_pages",
+    "b200_fork_workspace_bytes",
+    "b200_fork_sequences",
+    "b200_free_sequences",
+    "b200_keep_accepted",
     "b200_device_error",
     "b200_wait_selftest",
 )
@@ -155,6 +169,48 @@ class KvDequantParams(ctypes.Structure):
     ]
 
 
+class PromptAttnParams(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p),
+        ("cu_seqlens_q", c_void_p), ("cu_seqlens_k", c_void_p),
+        ("q_stride_t", i64), ("q_stride_h", i64), ("k_stride_t", i64), ("k_stride_h", i64),
+        ("v_stride_t", i64), ("v_stride_h", i64), ("out_stride_t", i64), ("out_stride_h", i64),
+        ("seqlen_dtype", i32), ("dtype", i32), ("num_seqs", i32), ("total_q", i32), ("total_k", i32),
+        ("num_q_heads", i32), ("num_kv_heads", i32), ("head_dim", i32), ("max_seqlen_k", i32), ("causal", i32),
+        ("softmax_scale", ctypes.c_float), ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class TreeAttnParams(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("tree_mask", c_void_p),
+        ("block_table", c_void_p), ("cu_seqlens_q", c_void_p), ("seqused_k", c_void_p),
+        ("q_stride_t", i64), ("q_stride_h", i64),
+        ("k_stride_block", i64), ("k_stride_tok", i64), ("k_stride_head", i64),
+        ("v_stride_block", i64), ("v_stride_tok", i64), ("v_stride_head", i64),
+        ("out_stride_t", i64), ("out_stride_h", i64), ("mask_stride", i64), ("block_table_stride", i64),
+        ("mask_cols", i32), ("block_table_cols", i32), ("block_table_dtype", i32), ("seqlen_dtype", i32),
+        ("dtype", i32), ("num_seqs", i32), ("total_q", i32), ("num_q_heads", i32), ("num_kv_heads", i32),
+        ("head_dim", i32), ("block_size", i32), ("num_blocks", i32), ("max_seqlen_k", i32),
+        ("softmax_scale", ctypes.c_float), ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PageCaches(ctypes.Structure):
+    _fields_ = [
+        ("base", c_void_p), ("num_caches", i32), ("num_blocks", i32), ("block_size", i32), ("num_kv_heads", i32),
+        ("row_bytes", i64), ("stride_block", i64), ("stride_tok", i64), ("stride_head", i64),
+    ]
+
+
+class SeqTable(ctypes.Structure):
+    _fields_ = [
+        ("block_table", c_void_p), ("seq_lens", c_void_p), ("ref_counts", c_void_p), ("stride", i64),
+        ("cols", i32), ("max_seqs", i32), ("num_blocks", i32), ("block_size", i32),
+        ("table_dtype", i32), ("seqlen_dtype", i32),
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -194,6 +250,23 @@ def load() -> ctypes.CDLL:
         lib.b200_kv_cache_write.argtypes = [ctypes.POINTER(KvWriteParams), c_void_p]
         lib.b200_kv_dequant_pages.restype = ctypes.c_int
         lib.b200_kv_dequant_pages.argtypes = [ctypes.POINTER(KvDequantParams), c_void_p]
+        lib.b200_varlen_attn_workspace_bytes.restype = ctypes.c_size_t
+        lib.b200_varlen_attn_workspace_bytes.argtypes = [i32] * 6
+        lib.b200_prompt_attn_fwd.restype = ctypes.c_int
+        lib.b200_prompt_attn_fwd.argtypes = [ctypes.POINTER(PromptAttnParams), c_void_p]
+        lib.b200_tree_attn_fwd.restype = ctypes.c_int
+        lib.b200_tree_attn_fwd.argtypes = [ctypes.POINTER(TreeAttnParams), c_void_p]
+        caches, table = ctypes.POINTER(PageCaches), ctypes.POINTER(SeqTable)
+        lib.b200_copy_pages.restype = ctypes.c_int
+        lib.b200_copy_pages.argtypes = [caches, c_void_p, c_void_p, i32, i32, c_void_p]
+        lib.b200_fork_workspace_bytes.restype = ctypes.c_size_t
+        lib.b200_fork_workspace_bytes.argtypes = [i32, i32]
+        lib.b200_fork_sequences.restype = ctypes.c_int
+        lib.b200_fork_sequences.argtypes = [caches, table, c_void_p, c_void_p, i32, i32, c_void_p, ctypes.c_size_t, c_void_p]
+        lib.b200_free_sequences.restype = ctypes.c_int
+        lib.b200_free_sequences.argtypes = [table, c_void_p, i32, i32, c_void_p]
+        lib.b200_keep_accepted.restype = ctypes.c_int
+        lib.b200_keep_accepted.argtypes = [caches, table, c_void_p, c_void_p, i64, i32, c_void_p, i32, c_void_p]
         lib.b200_device_error.restype = ctypes.c_int
         lib.b200_device_error.argtypes = [c_void_p, ctypes.POINTER(ctypes.c_uint32)]
         lib.b200_wait_selftest.restype = ctypes.c_int
@@ -223,6 +296,29 @@ def check(status: int, what: str) -> None:
 
 def current_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is current; nothing to enter or leave where it is already."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return _NO_SWITCH
+    return torch.cuda.device(device)
+
+
+def row_strides(t: torch.Tensor, strides: tuple) -> tuple[int, int]:
+    """(row, head) strides of ``[rows, heads, D]``; a dimension of one element counts as packed."""
+    sh = strides[1] if t.shape[1] != 1 else t.shape[2]
+    return (strides[0] if t.shape[0] != 1 else t.shape[1] * sh), sh
+
+
+def page_strides(t: torch.Tensor, strides: tuple) -> tuple[int, int, int]:
+    """(block, token, head) strides of ``[blocks, block, heads, D]``; a dimension of one element counts as packed."""
+    sh = strides[2] if t.shape[2] != 1 else t.shape[3]
+    return (strides[0] if t.shape[0] != 1 else t.shape[1] * strides[1]), strides[1], sh
 
 
 def device_error(device: torch.device | None = None) -> int:

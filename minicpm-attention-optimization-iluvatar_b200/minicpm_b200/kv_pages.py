@@ -1,0 +1,251 @@
+"""Page operators of a paged KV cache on sm_100a: copy, fork, free, keep.
+
+For serving that branches: parallel samples and beams share their prompt's pages
+(:func:`fork_sequences`, :func:`free_sequences`), a scheduler duplicates pages before
+they are written to (:func:`copy_pages`), and speculative decoding keeps the accepted
+path of a draft (:func:`keep_accepted_tokens`).  Every call serves all layers in one
+launch, on the current CUDA stream, without a host synchronisation, and can be
+captured in a CUDA graph.  No counterpart in the reference.
+
+A pool's state is three tensors that the caller owns: ``block_table [max_seqs,
+max_pages]`` (-1 = no page), ``seq_lens [max_seqs]`` and ``ref_counts [num_blocks]``
+(int32, how many rows of the table name a page; 0 = free).  What a call cannot serve
+(an index out of range, no page left) is skipped, leaves the other entries alone, and
+is recorded in the device error word (``minicpm_b200._lib.device_error()``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Union
+
+import torch
+
+from . import _lib
+
+
+class CacheLayers:
+    """The K and V tensors of a model's layers, checked once (:func:`cache_layers`).
+
+    Holds the tensors, so their memory stays valid; what is written to them later is
+    seen by every call.
+    """
+
+    def __init__(self, kv_caches: Sequence[torch.Tensor]):
+        views: list[torch.Tensor] = []
+        for cache in kv_caches:
+            if cache.ndim == 5 and cache.shape[1] == 2:
+                views += [cache[:, 0], cache[:, 1]]
+            elif cache.ndim == 4:
+                views.append(cache)
+            else:
+                raise ValueError("a cache is [num_blocks, 2, block_size, kv_heads, D] or [num_blocks, block_size, kv_heads, D]")
+        if not 1 <= len(views) <= 256:
+            raise ValueError("1 to 256 K/V tensors (128 layers) in one set of caches")
+        first = views[0]
+        for t in views:
+            if t.shape != first.shape or t.stride() != first.stride() or t.dtype != first.dtype or t.device != first.device:
+                raise ValueError("all caches must share shape, strides, dtype and device")
+        if first.numel() == 0 or (first.stride(3) != 1 and first.shape[3] != 1):
+            raise ValueError("the caches must not be empty and their rows must be contiguous")
+        if len({t.data_ptr() for t in views}) != len(views):
+            raise ValueError("a cache is named twice")
+        n, block, heads, row = first.shape
+        sb, st, sh, _ = first.stride()
+        row_run = row
+        page = block * heads * row
+        nhd = (heads == 1 or sh == row_run) and (block == 1 or st == heads * row_run)
+        hnd = (block == 1 or st == row_run) and (heads == 1 or sh == block * row_run)
+        if not (nhd or hnd) or (n > 1 and sb < page):
+            raise ValueError("a page must be one dense run of [block_size, kv_heads, D] or [kv_heads, block_size, D]")
+        e = first.element_size()
+        if n == 1:
+            sb = page
+        # A dimension of one element may carry any stride: the library gets the dense one.
+        if block == 1:
+            st = heads * row_run if nhd else row_run
+        if heads == 1:
+            sh = row_run
+        if (page * e) % 4 or (sb * e) % 4 or (row * e) % 4 or any(t.data_ptr() % 4 for t in views):
+            raise ValueError("cache rows must be 4-byte aligned")
+        self.tensors = list(kv_caches)
+        self.device = first.device
+        self.num_blocks, self.block_size = n, block
+        self._base = (ctypes.c_void_p * len(views))(*(t.data_ptr() for t in views))
+        self.params = _lib.PageCaches(ctypes.cast(self._base, ctypes.c_void_p), len(views), n, block, heads, row * e,
+                                      sb * e, st * e, sh * e)
+        self._ref = ctypes.byref(self.params)
+
+
+Caches = Union[CacheLayers, Sequence[torch.Tensor]]
+
+
+def cache_layers(kv_caches: Caches) -> CacheLayers:
+    """Check a model's caches once and keep them together for the calls below.
+
+    ``kv_caches``: one ``[num_blocks, 2, block_size, kv_heads, D]`` tensor per layer, or K and
+    V tensors ``[num_blocks, block_size, kv_heads, D]``; of one shape, one layout (NHD, or a
+    permuted view of HND) and any element type, quantised ones included (rows are moved with
+    the scale that they carry inline).
+    """
+    return kv_caches if isinstance(kv_caches, CacheLayers) else CacheLayers(kv_caches)
+
+
+def _indices(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if t.ndim != 1 or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be a one-dimensional int32 or int64 tensor")
+    if t.device != device:
+        raise ValueError(f"{name} must be on the same device as the table or caches")
+    return t.contiguous()
+
+
+def _table(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: Optional[torch.Tensor], num_blocks: int,
+           block_size: int) -> "_lib.SeqTable":
+    dev = block_table.device
+    if block_table.ndim != 2 or block_table.dtype not in (torch.int32, torch.int64) or block_table.shape[1] == 0:
+        raise ValueError("block_table must contain integer physical block ids, [max_seqs, max_pages]")
+    if block_table.stride(1) != 1 or (block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]):
+        raise ValueError("block_table is written in place: its rows must be contiguous and apart")
+    if seq_lens.ndim != 1 or seq_lens.shape[0] != block_table.shape[0] or seq_lens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("seq_lens must hold one int32 or int64 length per row of the block table")
+    if not seq_lens.is_contiguous():
+        raise ValueError("seq_lens is written in place: it must be contiguous")
+    if seq_lens.device != dev:
+        raise ValueError("block_table and seq_lens must be on the same device")
+    refs = None
+    if ref_counts is not None:
+        if ref_counts.ndim != 1 or ref_counts.dtype != torch.int32 or ref_counts.shape[0] != num_blocks:
+            raise ValueError("ref_counts must hold one int32 per page")
+        if not ref_counts.is_contiguous() or ref_counts.device != dev:
+            raise ValueError("ref_counts is written in place: contiguous, on the table's device")
+        refs = ref_counts.data_ptr()
+    return _lib.SeqTable(block_table.data_ptr(), seq_lens.data_ptr(), refs,
+                         max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], block_table.shape[0],
+                         num_blocks, block_size, _lib.dtype_code(block_table.dtype), _lib.dtype_code(seq_lens.dtype))
+
+
+def _same_device(layers: CacheLayers, dev: torch.device) -> None:
+    if layers.device != dev:
+        raise ValueError("the caches and the indices must be on the same device")
+
+
+def _cuda(dev: torch.device, what: str) -> None:
+    if dev.type != "cuda":
+        raise RuntimeError(f"{what} runs on CUDA tensors only (no CPU path)")
+
+
+def copy_pages(kv_caches: Caches, src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
+    """Copy page ``src_pages[i]`` to page ``dst_pages[i]`` in every layer's K and V.
+
+    A pair with a negative index is padding.  A destination may be neither named twice nor
+    a source of another pair: the copies run at the same time.
+    """
+    layers = cache_layers(kv_caches)
+    dev = layers.device
+    src, dst = _indices("src_pages", src_pages, dev), _indices("dst_pages", dst_pages, dev)
+    if src.shape != dst.shape or src.dtype != dst.dtype:
+        raise ValueError("src_pages and dst_pages must have one length and dtype")
+    _cuda(dev, "copy_pages")
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        _lib.check(lib.b200_copy_pages(layers._ref, src.data_ptr(), dst.data_ptr(), src.shape[0],
+                                       _lib.dtype_code(src.dtype), _lib.current_stream(dev)), "copy_pages")
+
+
+def fork_sequences(kv_caches: Caches, block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor,
+                   parents: torch.Tensor, children: torch.Tensor) -> None:
+    """Make row ``children[i]`` of the table a copy of row ``parents[i]``, for every ``i``.
+
+    Full pages are shared and their counts rise; the used rows of a partial last page are
+    copied, in every layer, to a page of the child's own: the lowest free pages, given out in
+    the order of the entries.  The child's row must be empty (length 0) and is named once; a
+    parent may have any number of children.  Entries with a negative index are padding; one
+    that cannot be served leaves its child empty and is recorded.
+    """
+    layers = cache_layers(kv_caches)
+    dev = layers.device
+    table = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)
+    _same_device(layers, block_table.device)
+    if ref_counts is None:
+        raise ValueError("fork_sequences needs ref_counts")
+    p, c = _indices("parents", parents, dev), _indices("children", children, dev)
+    if p.shape != c.shape or p.dtype != c.dtype:
+        raise ValueError("parents and children must have one length and dtype")
+    _cuda(dev, "fork_sequences")
+    n = p.shape[0]
+    if n == 0:
+        return
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        nbytes = lib.b200_fork_workspace_bytes(n, block_table.shape[0])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.check(lib.b200_fork_sequences(layers._ref, ctypes.byref(table), p.data_ptr(), c.data_ptr(), n,
+                                           _lib.dtype_code(p.dtype), ws.data_ptr(), nbytes, _lib.current_stream(dev)),
+                   "fork_sequences")
+
+
+def free_sequences(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor,
+                   rows: torch.Tensor) -> None:
+    """Empty the rows named: their pages' counts fall, their entries become -1, their lengths 0.
+
+    A page whose count reaches 0 is free.  Naming a row twice, or an empty one, releases
+    nothing twice; negative rows are padding.
+    """
+    dev = block_table.device
+    if ref_counts is None:
+        raise ValueError("free_sequences needs ref_counts")
+    table = _table(block_table, seq_lens, ref_counts, max(int(ref_counts.numel()), 1), 1)
+    r = _indices("rows", rows, dev)
+    _cuda(dev, "free_sequences")
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        _lib.check(lib.b200_free_sequences(ctypes.byref(table), r.data_ptr(), r.shape[0], _lib.dtype_code(r.dtype),
+                                           _lib.current_stream(dev)), "free_sequences")
+
+
+def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_lens: torch.Tensor,
+                         accepted: torch.Tensor, num_accepted: torch.Tensor, seq_lens: torch.Tensor,
+                         ref_counts: Optional[torch.Tensor] = None) -> None:
+    """Move the accepted drafted tokens of every sequence together, behind its context.
+
+    For row ``b`` and ``i < num_accepted[b]``, the K/V row at position ``context_lens[b] +
+    accepted[b, i]`` goes to ``context_lens[b] + i`` in every layer, and ``seq_lens[b]`` becomes
+    ``context_lens[b] + num_accepted[b]``.  ``accepted`` ``[num_seqs, A]`` holds the path's indices
+    among the drafted tokens, strictly rising; what is behind ``num_accepted[b]`` is not read.
+    With ``ref_counts`` the pages behind the new lengths are released (their table entries
+    become -1) and a shared page is not written to.  A path is cut before its first entry
+    that does not rise or has no page of its own, which is recorded.
+    """
+    layers = cache_layers(kv_caches)
+    dev = layers.device
+    table = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)
+    _same_device(layers, block_table.device)
+    if context_lens.shape != seq_lens.shape or context_lens.dtype != seq_lens.dtype or context_lens.device != dev:
+        raise ValueError("context_lens must match seq_lens")
+    if accepted.ndim != 2 or accepted.shape[0] != block_table.shape[0] or accepted.device != dev:
+        raise ValueError("accepted must have one row per row of the block table")
+    counts = _indices("num_accepted", num_accepted, dev)
+    if counts.shape[0] != accepted.shape[0] or counts.dtype != accepted.dtype:
+        raise ValueError("num_accepted must hold one count per row, in the dtype of accepted")
+    if context_lens.numel() and context_lens.data_ptr() == seq_lens.data_ptr():
+        raise ValueError("seq_lens may not be context_lens")
+    _cuda(dev, "keep_accepted_tokens")
+    if accepted.shape[1] and (accepted.stride(1) != 1 or accepted.stride(0) < accepted.shape[1]):
+        accepted = accepted.contiguous()
+    context_lens = context_lens.contiguous()
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        _lib.check(lib.b200_keep_accepted(layers._ref, ctypes.byref(table), context_lens.data_ptr(), accepted.data_ptr(),
+                                          max(accepted.stride(0), accepted.shape[1]), accepted.shape[1],
+                                          counts.data_ptr(), _lib.dtype_code(counts.dtype), _lib.current_stream(dev)),
+                   "keep_accepted_tokens")
+
+
+__all__ = [
+    "CacheLayers",
+    "cache_layers",
+    "copy_pages",
+    "fork_sequences",
+    "free_sequences",
+    "keep_accepted_tokens",
+]

@@ -1,0 +1,114 @@
+"""Attention of drafted token trees over a paged cache on sm_100a.
+
+Speculative decoding verifies the drafted tokens of every sequence in one pass:
+their K/V rows are written to the cache behind the context (as any new token's),
+and each token attends to the context and to its own ancestors in the tree.  One
+call of ``b200_tree_attn_fwd``: a device-side work list, the tcgen05 attention kernel
+in its form for trees, and a combine of split keys, on the current CUDA stream
+without a host synchronisation.  No counterpart in the reference.
+:func:`minicpm_b200.kv_pages.keep_accepted_tokens` then moves the accepted path
+together in the cache.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+
+def paged_tree_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    tree_mask: torch.Tensor,
+    block_table: torch.Tensor,
+    seqused_k: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    softmax_scale: float,
+) -> torch.Tensor:
+    """Attend the drafted tokens of every sequence to its context and their tree; returns ``out``.
+
+    ``q``/``out`` ``[T, Hq, D]``, the caches ``k``/``v`` ``[num_blocks, block_size, KH, D]``,
+    ``block_table``, ``seqused_k`` and ``cu_seqlens_q`` as in
+    :func:`~minicpm_b200.paged_split_kv_attention`.  The last ``n = cu_seqlens_q[b + 1] -
+    cu_seqlens_q[b]`` of the ``seqused_k[b]`` cached tokens of sequence ``b`` are its
+    drafted ones.  ``tree_mask`` ``[T, W]`` (bool or uint8, W >= ``max_seqlen_q``): row ``t``
+    sees drafted token ``j`` of its sequence iff ``tree_mask[t, j]``; it sees every token of
+    the context.  A drafted token usually sees itself and its ancestors, but any mask goes;
+    a row that sees nothing is 0.  Rows of ``out`` that belong to no sequence are left as
+    they were.  Cached keys and values of a sequence must be finite, those past its length
+    may hold anything.  A lower-triangular mask gives causal attention; one token per
+    sequence with ``tree_mask[t, 0]`` set is a decode step.
+    """
+    if q.ndim != 3 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError("expected q=[T,H,D] and k/v=[blocks,block,kv_heads,D]")
+    if out.shape != q.shape or k.shape != v.shape:
+        raise ValueError("out must match q and k/v must have identical shapes")
+    dev = q.device
+    for t in (k, v, out, tree_mask, block_table, seqused_k, cu_seqlens_q):
+        if t.device != dev:
+            raise ValueError("all tensors must be on the same device")
+    if block_table.ndim != 2 or block_table.dtype not in (torch.int32, torch.int64):
+        raise ValueError("block_table must contain integer physical block ids")
+    if cu_seqlens_q.ndim != 1 or seqused_k.ndim != 1:
+        raise ValueError("cu_seqlens_q and seqused_k must be one-dimensional")
+    num_seqs = seqused_k.shape[0]
+    if cu_seqlens_q.shape[0] != num_seqs + 1:
+        raise ValueError("cu_seqlens_q must contain one entry per request plus one")
+    if block_table.shape[0] != num_seqs:
+        raise ValueError("block_table and seqused_k must have the same request count")
+    if cu_seqlens_q.dtype != seqused_k.dtype or cu_seqlens_q.dtype not in (torch.int32, torch.int64):
+        raise ValueError("cu_seqlens_q and seqused_k must be int32 or int64 of one dtype")
+    total_q, hq, head_dim = q.shape
+    num_blocks, block_size, hkv, dk = k.shape
+    if (dk != head_dim or head_dim not in (64, 128, 256) or hkv == 0 or hq == 0 or hq % hkv or block_size <= 0
+            or block_size % 16):
+        raise ValueError("unsupported head shape for tree attention")
+    if tree_mask.ndim != 2 or tree_mask.shape[0] != total_q or tree_mask.dtype not in (torch.bool, torch.uint8):
+        raise ValueError("tree_mask must be bool or uint8 with one row per query token")
+    if tree_mask.shape[1] < max_seqlen_q:
+        raise ValueError("tree_mask must have a column for each of the max_seqlen_q drafted tokens")
+    if not softmax_scale > 0.0 or softmax_scale > 3.0e38:
+        raise ValueError("softmax_scale must be positive and finite")
+    if dev.type != "cuda":
+        raise RuntimeError("paged_tree_attention runs on CUDA tensors only (no CPU path)")
+    dtype = q.dtype
+    if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
+        raise RuntimeError("the sm_100a kernel takes bf16 or f16 q/k/v/out of one dtype")
+    qs, ks, vs, outs = q.stride(), k.stride(), v.stride(), out.stride()
+    if qs[2] != 1 or ks[3] != 1 or vs[3] != 1 or outs[2] != 1:
+        raise RuntimeError("the head dimension of q, k, v and out must be contiguous")
+    if num_blocks == 0 or block_table.shape[1] == 0:
+        raise ValueError("the cache and the block table must have at least one page")
+    if total_q == 0 or num_seqs == 0:
+        return out
+    if tree_mask.stride(1) != 1:
+        tree_mask = tree_mask.contiguous()
+    if block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    cu_seqlens_q = cu_seqlens_q.contiguous()
+    seqused_k = seqused_k.contiguous()
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        nbytes = lib.b200_varlen_attn_workspace_bytes(total_q, num_seqs, hq, hkv, head_dim, int(max_seqlen_k))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        p = _lib.TreeAttnParams(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), tree_mask.data_ptr(), block_table.data_ptr(),
+            cu_seqlens_q.data_ptr(), seqused_k.data_ptr(),
+            *_lib.row_strides(q, qs), *_lib.page_strides(k, ks), *_lib.page_strides(v, vs), *_lib.row_strides(out, outs),
+            tree_mask.stride(0), block_table.stride(0), tree_mask.shape[1], block_table.shape[1],
+            _lib.dtype_code(block_table.dtype), _lib.dtype_code(seqused_k.dtype), _lib.dtype_code(dtype), num_seqs,
+            total_q, hq, hkv, head_dim, block_size, num_blocks, int(max_seqlen_k), float(softmax_scale),
+            ws.data_ptr(), nbytes,
+        )
+        _lib.check(lib.b200_tree_attn_fwd(ctypes.byref(p), _lib.current_stream(dev)), "paged_tree_attention")
+    return out
+
+
+__all__ = ["paged_tree_attention"]

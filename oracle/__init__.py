@@ -29,6 +29,7 @@ from .kv_cache import (
     rope_and_cache_service_reference,
 )
 from .rope import reference_rope, rope_and_cache_reference, rotate_fp32
+from .varlen_attention import attention_tolerance, prompt_attention_reference, tree_attention_reference
 
 __all__ = [
     "causal_flops",
@@ -45,4 +46,7 @@ __all__ = [
     "quantize_per_token_head",
     "kv_write_reference",
     "rope_and_cache_service_reference",
+    "attention_tolerance",
+    "prompt_attention_reference",
+    "tree_attention_reference",
 ]
