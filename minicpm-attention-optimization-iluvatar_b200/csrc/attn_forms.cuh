@@ -1,11 +1,11 @@
 // attn_forms.cuh -- launch of the attention kernel's bounded forms
-// (kFormPrompt, kFormTree): workspace, split bound, schedule, attention,
-// combine of split units.
+// (kFormPrompt, kFormTree): workspace, division of the work, attention, join of
+// shared units.
 //
 // The form runs paged_attn_fwd_kernel's pipeline; what differs from the causal
 // paged call is here and in the kForm branches of that kernel.  Partial outputs
-// of split units are fp32, so a split costs no rounding: the result is rounded
-// once, when the combine (or the unsplit epilogue) stores it.
+// of shared units are fp32, so sharing costs no rounding: the result is rounded
+// once, when the join (or the epilogue of a whole unit) stores it.
 #pragma once
 
 #include <algorithm>
@@ -17,114 +17,111 @@
 
 namespace b200 {
 
-// The most runs one query unit's keys are split into.  A draft batch of one
-// sequence has as few as KH units for 148 SMs; 64 runs of at least
-// kMinSplitTiles tiles keep every SM busy from 2 KV heads x 16K keys on.
-constexpr int kMaxFormSplits = 64;
-
-struct FormCombineArgs {
-  const float* o_part;    // [slots][num_splits][kUnitRows][D], normalised
-  const float* m_part;    // [slots][num_splits][kUnitRows]
+struct StreamCombineArgs {
+  const int4* meta;       // [CTAs]: sequence, query unit, KV head, pieces of the unit that CTA i began (0: none)
+  const float* o_part;    // [2 CTAs][D / 4][kUnitRows][4], normalised
+  const float* m_part;    // [2 CTAs][kUnitRows]
   const float* l_part;
-  const int4* split_units;
-  const int* unit_count;  // [2] = slots
   const void* cu_q;
   void* out;
   int64_t out_st, out_sh;
   int len_i64, total_q;
-  int num_splits, group, pos_per_tile, pos_per_unit;
+  int group, pos_per_tile, pos_per_unit;
 };
 
-// out = sum_s w_s O_s / sum_s w_s, w_s = exp(m_s - max m) l_s, over the runs of a
-// split unit: D / 8 threads a row, the m / l of a row loaded once per group and
-// the weights passed by shuffles, four runs' O in flight per thread.  Memory
-// bound; a call without split units ends at once.
+// out = sum_s w_s O_s / sum_s w_s, w_s = exp(m_s - max m) l_s, over the pieces of a
+// unit that streamed CTAs share: the first in slot 2 i + 1, the others in the slots
+// 2 (i + 1), 2 (i + 2), .. of the CTAs behind.  A block joins 32 rows of CTA i's
+// unit: lane r of warp w has row r and the column quads w, w + 8, .., so that every
+// load of a warp is one run of 512 bytes, with the pieces of kJoinRun slots in
+// flight; the rows leave through shared memory as 16-byte pieces.  Latency and L2
+// bound (the partials were just written); a CTA that shares no unit costs one load.
+constexpr int kJoinRows = 32;
+template <int D>
+constexpr int kJoinRun = D == 64 ? 8 : D == 128 ? 4 : 2;
+
 template <typename T, int D, int kForm>
-__global__ void __launch_bounds__(kCombineThreads) form_combine_kernel(const FormCombineArgs a) {
-  constexpr int kTpr = D / 8;  // threads per row: 8, 16 or 32, so a warp's rows belong to one unit
-  constexpr int kRowsPerBlock = kCombineThreads / kTpr;
-  constexpr int kPer = kMaxFormSplits / kTpr;
+__global__ void __launch_bounds__(kCombineThreads) stream_combine_kernel(const StreamCombineArgs a) {
+  constexpr int kWarps = kCombineThreads / 32;
+  constexpr int kQuads = D / 4 / kWarps;  // column quads of a lane
+  constexpr int kRun = kJoinRun<D>;
+  __shared__ uint2 rows[kJoinRows][D / 4 + 1];
   griddep_wait();
-  const int sub = threadIdx.x % kTpr;
-  const int64_t rows = static_cast<int64_t>(a.unit_count[2]) * kUnitRows;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock; base < rows;
-       base += static_cast<int64_t>(gridDim.x) * kRowsPerBlock) {
-    // rows is a multiple of 256, so every row of the block exists
-    const int64_t row = base + threadIdx.x / kTpr;
-    const int slot = static_cast<int>(row / kUnitRows);
-    const int ur = static_cast<int>(row - static_cast<int64_t>(slot) * kUnitRows);
-    const int4 su = a.split_units[slot];  // (seq, qunit, kvh, splits)
+  const int cta = blockIdx.x;
+  const int4 su = a.meta[cta];
+  if (su.w == 0) return;
+  const int q_begin = min(max(load_index(a.cu_q, su.x, a.len_i64), 0), a.total_q);
+  const int q_end = min(load_index(a.cu_q, su.x + 1, a.len_i64), a.total_q);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto place = [&](int ur, int64_t& tok, int64_t& head) -> bool {  // where row ur of the unit goes, if it exists
     const int t = ur / kAttnTileM, r = ur % kAttnTileM;
-    const int q_begin = min(max(load_index(a.cu_q, su.x, a.len_i64), 0), a.total_q);
-    const int q_end = min(load_index(a.cu_q, su.x + 1, a.len_i64), a.total_q);
     const int pos = su.y * a.pos_per_unit + t * a.pos_per_tile + r / a.group;
-    const bool valid = r < a.group * a.pos_per_tile && t * a.pos_per_tile < a.pos_per_unit && pos < q_end - q_begin;
-    if (!__any_sync(0xffffffffu, valid)) continue;
-    const int n = su.w;
-    const int64_t prow = static_cast<int64_t>(slot) * a.num_splits * kUnitRows + ur;
-    float mk[kPer], wk[kPer], m_max = -INFINITY;
+    tok = q_begin + pos;
+    head = static_cast<int64_t>(su.z) * a.group + r % a.group;
+    return r < a.group * a.pos_per_tile && t * a.pos_per_tile < a.pos_per_unit && pos < q_end - q_begin;
+  };
+  const int ur = blockIdx.y * kJoinRows + lane;
+  int64_t tok, head;
+  const bool valid = place(ur, tok, head);
+  if (!__any_sync(0xffffffffu, valid)) return;  // the same in every warp
+  float m_max = -INFINITY, den = 0.f;
+  float acc[kQuads][4] = {};
+  for (int s0 = 0; s0 < su.w; s0 += kRun) {
+    float m[kRun], l[kRun];
+    float4 x[kRun][kQuads];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int s = sub + k * kTpr;
-      const bool has = valid && s < n;
-      mk[k] = has ? a.m_part[prow + static_cast<int64_t>(s) * kUnitRows] : -INFINITY;
-      wk[k] = has ? a.l_part[prow + static_cast<int64_t>(s) * kUnitRows] : 0.f;
-      m_max = fmaxf(m_max, mk[k]);
-    }
+    for (int k = 0; k < kRun; ++k) {
+      const int s = s0 + k;
+      m[k] = -INFINITY;
+      l[k] = 0.f;
+      if (valid && s < su.w) {
+        const int64_t slot = 2 * (cta + s) + (s == 0 ? 1 : 0);
+        m[k] = a.m_part[slot * kUnitRows + ur];
+        l[k] = a.l_part[slot * kUnitRows + ur];
+        const float4* p = reinterpret_cast<const float4*>(a.o_part) + slot * (D / 4) * kUnitRows + ur;
 #pragma unroll
-    for (int off = kTpr / 2; off > 0; off >>= 1) m_max = fmaxf(m_max, __shfl_xor_sync(0xffffffffu, m_max, off, kTpr));
-    float den = 0.f;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      // A run in which the row saw no key has l = 0 and its O is left out by
-      // selection.  A NaN among the row's scores makes l NaN: it is kept.
-      wk[k] = wk[k] != 0.f ? expf(mk[k] - m_max) * wk[k] : -1.f;
-      if (!(wk[k] < 0.f)) den += wk[k];
-    }
-#pragma unroll
-    for (int off = kTpr / 2; off > 0; off >>= 1) den += __shfl_xor_sync(0xffffffffu, den, off, kTpr);
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const float* o = a.o_part + prow * D + sub * 8;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      if (k * kTpr >= n) break;  // the same in the whole warp
-#pragma unroll 1
-      for (int j = 0; j < kTpr; j += 4) {
-        float w[4];
-        float4 x[4], y[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int s = k * kTpr + j + u;
-          w[u] = __shfl_sync(0xffffffffu, wk[k], j + u, kTpr);
-          x[u] = y[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (valid && s < n && !(w[u] < 0.f)) {
-            const float4* p = reinterpret_cast<const float4*>(o + static_cast<int64_t>(s) * kUnitRows * D);
-            x[u] = __ldcs(p);
-            y[u] = __ldcs(p + 1);
-          } else {
-            w[u] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          acc[0] = fmaf(w[u], x[u].x, acc[0]);
-          acc[1] = fmaf(w[u], x[u].y, acc[1]);
-          acc[2] = fmaf(w[u], x[u].z, acc[2]);
-          acc[3] = fmaf(w[u], x[u].w, acc[3]);
-          acc[4] = fmaf(w[u], y[u].x, acc[4]);
-          acc[5] = fmaf(w[u], y[u].y, acc[5]);
-          acc[6] = fmaf(w[u], y[u].z, acc[6]);
-          acc[7] = fmaf(w[u], y[u].w, acc[7]);
-        }
+        for (int c = 0; c < kQuads; ++c) x[k][c] = p[(warp + c * kWarps) * kUnitRows];
       }
     }
-    const float inv = den == 0.f ? 0.f : 1.f / den;
+    float m_new = m_max;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] *= inv;
-    if (valid) {
-      const int64_t tok = q_begin + pos, head = static_cast<int64_t>(su.z) * a.group + r % a.group;
-      store8<T>(static_cast<T*>(a.out) + tok * a.out_st + head * a.out_sh + sub * 8, acc);
+    for (int k = 0; k < kRun; ++k) m_new = fmaxf(m_new, m[k]);
+    const float scale = m_max == -INFINITY ? 0.f : expf(m_max - m_new);
+    den *= scale;
+#pragma unroll
+    for (int c = 0; c < kQuads; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[c][i] *= scale;
+    m_max = m_new;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      // A piece in which the row saw no key has l = 0 and its O is left out by
+      // selection.  A NaN among the row's scores makes l NaN: it is kept.
+      if (l[k] == 0.f) continue;
+      const float w = expf(m[k] - m_max) * l[k];
+      den += w;
+#pragma unroll
+      for (int c = 0; c < kQuads; ++c) {
+        acc[c][0] = fmaf(w, x[k][c].x, acc[c][0]);
+        acc[c][1] = fmaf(w, x[k][c].y, acc[c][1]);
+        acc[c][2] = fmaf(w, x[k][c].z, acc[c][2]);
+        acc[c][3] = fmaf(w, x[k][c].w, acc[c][3]);
+      }
     }
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+  for (int c = 0; c < kQuads; ++c)
+    rows[lane][warp + c * kWarps] = make_uint2(Pack2<T>::pack(acc[c][0] * inv, acc[c][1] * inv),
+                                               Pack2<T>::pack(acc[c][2] * inv, acc[c][3] * inv));
+  __syncthreads();
+  constexpr int kPieces = D / 8;  // 16-byte pieces of a row
+  for (int i = threadIdx.x; i < kJoinRows * kPieces; i += kCombineThreads) {
+    const int r = i / kPieces, c = i % kPieces;
+    if (!place(blockIdx.y * kJoinRows + r, tok, head)) continue;
+    const uint2 lo = rows[r][2 * c], hi = rows[r][2 * c + 1];
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.out_st + head * a.out_sh + c * 8) =
+        make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
 }
 
@@ -133,43 +130,53 @@ __global__ void __launch_bounds__(kCombineThreads) form_combine_kernel(const For
 namespace b200_host {
 
 struct FormLayout {
-  size_t count_off, tile_base_off, seq_off_off, qbase_off, qsplit_off, qslot_off, units_off, split_units_off;
-  size_t o_off, m_off, l_off, total;
-  int ppt, ppu, splits;
-  int64_t qunits_ub, capacity, slots_ub;
+  bool streamed;
+  int ctas, ppt, ppu;
+  int64_t qunits_ub, capacity;
+  // streamed: CTAs' shared units and partials
+  size_t meta_off, o_off, m_off, l_off;
+  // listed: the schedule kernel's arrays
+  size_t count_off, tile_base_off, seq_off_off, qbase_off, qsplit_off, qslot_off, units_off;
+  size_t total;
 };
 
-// The bound on the splits of a unit: enough runs that the units the batch is
-// sure to have give every SM two, each run at least kMinSplitTiles tiles of the
-// longest sequence.  The schedule kernel then splits each unit by its share.
-inline FormLayout form_layout(int64_t total_q, int num_seqs, int hq, int hkv, int head_dim, int max_seqlen_k,
-                              int sms) {
+// Draft trees are always streamed.  Prompts are where whole units would leave SMs
+// idle: fewer units than SMs, or few rounds of long ones.  Elsewhere the list wins:
+// its dynamic claims balance better, and it writes no partials (33 sequences of up
+// to 517 tokens x 12 heads: 52 us listed, 74 us streamed).
+constexpr int kStreamRounds = 8;
+constexpr int kStreamLongTiles = 32;
+
+inline FormLayout form_layout(bool tree, int64_t total_q, int num_seqs, int hq, int hkv, int head_dim,
+                              int max_seqlen_k, int sms) {
   FormLayout w{};
   const int group = hq / hkv;
   w.ppt = b200::kAttnTileM / group;
   w.ppu = w.ppt * (head_dim == 256 ? 1 : b200::kAttnTilesPerUnit);
   w.qunits_ub = (total_q + w.ppu - 1) / w.ppu + num_seqs;
+  w.capacity = w.qunits_ub * hkv;
+  const int64_t tiles = std::max(max_seqlen_k, 0) / b200::kAttnTileN + 1;
+  const int64_t ticks = w.capacity * (b200::kStreamOverhead + 2 * tiles);
   const int64_t units_lb =
       std::max<int64_t>((total_q + w.ppu - 1) / w.ppu, std::min<int64_t>(num_seqs, total_q)) * hkv;
-  const int64_t most = std::max(max_seqlen_k, 1) / (b200::kMinSplitTiles * b200::kAttnTileN);
-  const int64_t want = (2 * (int64_t)sms + units_lb - 1) / std::max<int64_t>(units_lb, 1);
-  w.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)b200::kMaxFormSplits}));
-  w.capacity = w.qunits_ub * hkv * w.splits;
-  w.slots_ub = w.splits > 1 ? w.qunits_ub * hkv : 0;
+  w.streamed = tree || units_lb < sms || (units_lb < (int64_t)kStreamRounds * sms && tiles >= kStreamLongTiles);
+  w.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(w.streamed ? ticks / b200::kStreamMinTicks : w.capacity, sms));
+  if (w.streamed) {
+    const size_t rows = (size_t)2 * w.ctas * b200::kUnitRows;
+    w.o_off = align_up(sizeof(int4) * (size_t)w.ctas, 256);
+    w.m_off = w.o_off + rows * head_dim * sizeof(float);
+    w.l_off = w.m_off + rows * sizeof(float);
+    w.total = w.l_off + rows * sizeof(float);
+    return w;
+  }
   const size_t qn = (size_t)w.qunits_ub;
-  w.count_off = 0;
   w.tile_base_off = 256;
   w.seq_off_off = align_up(w.tile_base_off + sizeof(int) * ((size_t)num_seqs + 1), 256);
   w.qbase_off = align_up(w.seq_off_off + sizeof(int) * (size_t)num_seqs, 256);
   w.qsplit_off = align_up(w.qbase_off + sizeof(int) * (qn + 1), 256);
   w.qslot_off = align_up(w.qsplit_off + sizeof(int) * qn, 256);
   w.units_off = align_up(w.qslot_off + sizeof(int) * qn, 256);
-  w.split_units_off = align_up(w.units_off + sizeof(int4) * (size_t)w.capacity, 256);
-  w.o_off = align_up(w.split_units_off + sizeof(int4) * (size_t)w.slots_ub, 256);
-  const size_t rows = (size_t)w.slots_ub * (w.splits > 1 ? w.splits : 0) * b200::kUnitRows;
-  w.m_off = align_up(w.o_off + rows * head_dim * sizeof(float), 256);
-  w.l_off = align_up(w.m_off + rows * sizeof(float), 256);
-  w.total = align_up(w.l_off + rows * sizeof(float), 256);
+  w.total = align_up(w.units_off + sizeof(int4) * (size_t)w.capacity, 256);
   return w;
 }
 
@@ -206,11 +213,11 @@ int prepare_attn_kernel(Kernel kernel, std::atomic<uint64_t>& done) {
   return B200_OK;
 }
 
+// `dependent`: a programmatic dependent of the launch before it, whose end its
+// set-up overlaps; it waits (griddepcontrol.wait) before it reads that kernel's output.
 template <typename... KArgs, typename... Args>
-int launch_dependent(const char* what, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s,
-                     const Args&... args) {
-  // A programmatic dependent of the launch before it: its set-up overlaps that
-  // kernel's end, and it waits (griddepcontrol.wait) before it reads its output.
+int launch_form_kernel(const char* what, bool dependent, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem,
+                       cudaStream_t s, const Args&... args) {
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
@@ -220,7 +227,7 @@ int launch_dependent(const char* what, void (*kernel)(KArgs...), dim3 grid, int 
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = pdl;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = dependent ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kernel, args...);
   return check_launch(what);
 }
@@ -230,8 +237,8 @@ int launch_attn_form(const FormLaunch& f, dim3 grid, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto kernel = b200::paged_attn_fwd_kernel<T, kHeadMaps, kWide, kNarrow, kForm>;
   if (int r = prepare_attn_kernel(kernel, done)) return r;
-  return launch_dependent("attention kernel", kernel, grid, b200::kAttnThreads, b200::kAttnSmemAlloc, s, f.tm_q, f.maps,
-                          f.a);
+  return launch_form_kernel("attention kernel", !b200::form_streamed(kForm), kernel, grid, b200::kAttnThreads, b200::kAttnSmemAlloc, s,
+                            f.tm_q, f.maps, f.a);
 }
 
 template <typename T, bool kHeadMaps, int kForm>
@@ -242,26 +249,20 @@ int launch_attn_dim(const FormLaunch& f, dim3 grid, cudaStream_t s) {
 }
 
 template <typename T, int kForm>
-int launch_combine(const b200::FormCombineArgs& c, int head_dim, int64_t rows, int sms, cudaStream_t s) {
-  const int rows_per_block = b200::kCombineThreads / (head_dim / 8);
-  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((rows + rows_per_block - 1) / rows_per_block, (int64_t)sms * 8));
-  auto kernel = head_dim == 256  ? b200::form_combine_kernel<T, 256, kForm>
-                : head_dim == 64 ? b200::form_combine_kernel<T, 64, kForm>
-                                 : b200::form_combine_kernel<T, 128, kForm>;
-  return launch_dependent("form_combine_kernel", kernel, dim3((unsigned)blocks), b200::kCombineThreads, 0, s, c);
+int launch_combine(const b200::StreamCombineArgs& c, int head_dim, int ctas, cudaStream_t s) {
+  auto kernel = head_dim == 256  ? b200::stream_combine_kernel<T, 256, kForm>
+                : head_dim == 64 ? b200::stream_combine_kernel<T, 64, kForm>
+                                 : b200::stream_combine_kernel<T, 128, kForm>;
+  const unsigned chunks = b200::kUnitRows / b200::kJoinRows;
+  return launch_form_kernel("stream_combine_kernel", true, kernel, dim3((unsigned)ctas, chunks), b200::kCombineThreads, 0, s,
+                            c);
 }
 
+// The work list of kFormPrompt.
 template <int kForm>
-int run_form(FormLaunch& f, cudaStream_t s) {
-  b200::AttnKernelArgs& a = f.a;
-  const int sms = sm_count();
-  const FormLayout w = form_layout(a.total_q, f.num_seqs, a.num_q_heads, f.num_kv_heads, a.head_dim, f.max_seqlen_k, sms);
-  if (w.capacity > 0x7fffffff) return fail(B200_ERR_UNSUPPORTED, "more than 2^31 work units in one call");
-  if (!f.workspace || f.workspace_bytes < w.total)
-    return fail(B200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", w.total, f.workspace_bytes);
-  if (!aligned16(f.workspace)) return fail(B200_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+int launch_schedule(const FormLaunch& f, const FormLayout& w, int sms, cudaStream_t s) {
+  const b200::AttnKernelArgs& a = f.a;
   uint8_t* ws = static_cast<uint8_t*>(f.workspace);
-
   b200::SchedArgs sa{};
   sa.cu_q = a.cu_q;
   sa.seqused = a.seqused;
@@ -270,13 +271,11 @@ int run_form(FormLaunch& f, cudaStream_t s) {
   sa.num_seqs = f.num_seqs;
   sa.pos_per_unit = w.ppu;
   sa.num_kv_heads = f.num_kv_heads;
-  sa.num_splits = w.splits;
+  sa.num_splits = 1;
   sa.num_sms = sms;
   sa.capacity = (int)w.capacity;
   sa.total_q = a.total_q;
   sa.total_k = a.total_k;
-  sa.bt_cols = a.bt_cols;
-  sa.block_size = a.block_size;
   sa.max_qunits = (int)w.qunits_ub;
   sa.full = a.full;
   sa.tile_base = reinterpret_cast<int*>(ws + w.tile_base_off);
@@ -285,52 +284,68 @@ int run_form(FormLaunch& f, cudaStream_t s) {
   sa.qunit_split = reinterpret_cast<int*>(ws + w.qsplit_off);
   sa.qunit_slot = reinterpret_cast<int*>(ws + w.qslot_off);
   sa.units = reinterpret_cast<int4*>(ws + w.units_off);
-  sa.split_units = reinterpret_cast<int4*>(ws + w.split_units_off);
   sa.unit_count = reinterpret_cast<int*>(ws + w.count_off);
   auto sched = b200::attn_schedule_kernel<kForm>;
   cudaError_t e = cudaFuncSetAttribute(sched, cudaFuncAttributeMaxDynamicSharedMemorySize, b200::kSchedSmemBytes);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "schedule kernel shared memory: %s", cudaGetErrorString(e));
   sched<<<1, b200::kSchedThreads, b200::kSchedSmemBytes, s>>>(sa);
-  if (int r = check_launch("attn_schedule_kernel")) return r;
+  return check_launch("attn_schedule_kernel");
+}
 
-  a.o_split = ws + w.o_off;
-  a.m_split = reinterpret_cast<float*>(ws + w.m_off);
-  a.l_split = reinterpret_cast<float*>(ws + w.l_off);
-  a.units = sa.units;
-  a.unit_count = sa.unit_count;
+// `w` lies in the workspace; max_tiles bounds the KV tiles of a sequence by the caller's sizes.
+template <int kForm>
+int run_form(FormLaunch& f, const FormLayout& w, int64_t max_tiles, int sms, cudaStream_t s) {
+  b200::AttnKernelArgs& a = f.a;
+  if (w.capacity * (b200::kStreamOverhead + 2 * max_tiles) > 0x7fffffff)
+    return fail(B200_ERR_UNSUPPORTED, "more than 2^30 KV tiles of work in one call");
+  if (!f.workspace || f.workspace_bytes < w.total)
+    return fail(B200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", w.total, f.workspace_bytes);
+  if (!aligned16(f.workspace)) return fail(B200_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(f.workspace);
   a.pos_per_tile = w.ppt;
-  a.num_splits = w.splits;
-  const dim3 grid((unsigned)std::min<int64_t>(w.capacity, sms));
+  a.num_seqs = f.num_seqs;
+  a.num_kv_heads = f.num_kv_heads;
+  a.num_splits = 1;
+  a.wide_out = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_st * 2) | (uintptr_t)(a.out_sh * 2)) & 31) == 0;
+  if constexpr (b200::form_streamed(kForm)) {
+    a.stream_meta = reinterpret_cast<int4*>(ws);
+    a.o_split = ws + w.o_off;
+    a.m_split = reinterpret_cast<float*>(ws + w.m_off);
+    a.l_split = reinterpret_cast<float*>(ws + w.l_off);
+  } else {
+    a.units = reinterpret_cast<int4*>(ws + w.units_off);
+    a.unit_count = reinterpret_cast<int*>(ws + w.count_off);
+    if (int r = launch_schedule<kForm>(f, w, sms, s)) return r;
+  }
+  const dim3 grid((unsigned)w.ctas);
   const bool bf16 = f.dtype == B200_DTYPE_BF16;
   int r;
-  if constexpr (kForm == b200::kFormPrompt) {
+  constexpr bool kMaps = !b200::form_rows(kForm);
+  if (kMaps && f.head_maps)
+    r = bf16 ? launch_attn_dim<__nv_bfloat16, kMaps, kForm>(f, grid, s) : launch_attn_dim<__half, kMaps, kForm>(f, grid, s);
+  else
     r = bf16 ? launch_attn_dim<__nv_bfloat16, false, kForm>(f, grid, s) : launch_attn_dim<__half, false, kForm>(f, grid, s);
-  } else if (f.head_maps) {
-    r = bf16 ? launch_attn_dim<__nv_bfloat16, true, kForm>(f, grid, s) : launch_attn_dim<__half, true, kForm>(f, grid, s);
-  } else {
-    r = bf16 ? launch_attn_dim<__nv_bfloat16, false, kForm>(f, grid, s) : launch_attn_dim<__half, false, kForm>(f, grid, s);
-  }
-  if (r != B200_OK || w.splits == 1) return r;
+  if (r != B200_OK || !b200::form_streamed(kForm) || w.ctas == 1) return r;  // one CTA shares no unit
 
-  b200::FormCombineArgs c{};
-  c.o_part = static_cast<const float*>(a.o_split);
-  c.m_part = a.m_split;
-  c.l_part = a.l_split;
-  c.split_units = sa.split_units;
-  c.unit_count = sa.unit_count;
-  c.cu_q = a.cu_q;
-  c.out = a.out;
-  c.out_st = a.out_st;
-  c.out_sh = a.out_sh;
-  c.len_i64 = a.len_i64;
-  c.total_q = a.total_q;
-  c.num_splits = w.splits;
-  c.group = a.group;
-  c.pos_per_tile = w.ppt;
-  c.pos_per_unit = w.ppu;
-  const int64_t rows = w.slots_ub * b200::kUnitRows;
-  return bf16 ? launch_combine<__nv_bfloat16, kForm>(c, a.head_dim, rows, sms, s)
-              : launch_combine<__half, kForm>(c, a.head_dim, rows, sms, s);
+  if constexpr (b200::form_streamed(kForm)) {
+    b200::StreamCombineArgs c{};
+    c.meta = a.stream_meta;
+    c.o_part = static_cast<const float*>(a.o_split);
+    c.m_part = a.m_split;
+    c.l_part = a.l_split;
+    c.cu_q = a.cu_q;
+    c.out = a.out;
+    c.out_st = a.out_st;
+    c.out_sh = a.out_sh;
+    c.len_i64 = a.len_i64;
+    c.total_q = a.total_q;
+    c.group = a.group;
+    c.pos_per_tile = w.ppt;
+    c.pos_per_unit = w.ppu;
+    r = bf16 ? launch_combine<__nv_bfloat16, kForm>(c, a.head_dim, w.ctas, s)
+             : launch_combine<__half, kForm>(c, a.head_dim, w.ctas, s);
+  }
+  return r;
 }
 
 // Checks that both forms share: element type, head shape, alignment, scale.

@@ -23,7 +23,9 @@ size_t b200_varlen_attn_workspace_bytes(int32_t total_q, int32_t num_seqs, int32
   if (total_q <= 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       num_q_heads / num_kv_heads > b200::kAttnTileM || head_dim <= 0)
     return 0;
-  return form_layout(total_q, num_seqs, num_q_heads, num_kv_heads, head_dim, max_seqlen_k, sm_count()).total;
+  const int sms = sm_count();
+  return std::max(form_layout(true, total_q, num_seqs, num_q_heads, num_kv_heads, head_dim, max_seqlen_k, sms).total,
+                  form_layout(false, total_q, num_seqs, num_q_heads, num_kv_heads, head_dim, max_seqlen_k, sms).total);
 }
 
 int b200_prompt_attn_fwd(const B200PromptAttnParams* p, void* stream) {
@@ -73,7 +75,13 @@ int b200_prompt_attn_fwd(const B200PromptAttnParams* p, void* stream) {
   a.block_size = 1;
   a.full = p->causal ? 0 : 1;
   a.scale_log2 = static_cast<float>(static_cast<double>(p->softmax_scale) * 1.4426950408889634);
-  return run_form<b200::kFormPrompt>(f, static_cast<cudaStream_t>(stream));
+  const int sms = sm_count();
+  const FormLayout w = form_layout(false, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim,
+                                   p->max_seqlen_k, sms);
+  const int64_t max_tiles = (int64_t)p->total_k / b200::kAttnTileN + 1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return w.streamed ? run_form<b200::kFormPromptStream>(f, w, max_tiles, sms, s)
+                    : run_form<b200::kFormPrompt>(f, w, max_tiles, sms, s);
 }
 
 }  // extern "C"

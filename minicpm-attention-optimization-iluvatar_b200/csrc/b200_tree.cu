@@ -100,7 +100,11 @@ int b200_tree_attn_fwd(const B200TreeAttnParams* p, void* stream) {
   a.mask_cols = p->mask_cols;
   a.full = 1;
   a.scale_log2 = static_cast<float>(static_cast<double>(p->softmax_scale) * 1.4426950408889634);
-  return run_form<b200::kFormTree>(f, static_cast<cudaStream_t>(stream));
+  const int sms = sm_count();
+  const FormLayout w = form_layout(true, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim,
+                                   p->max_seqlen_k, sms);
+  const int64_t max_tiles = (int64_t)p->block_table_cols * p->block_size / b200::kAttnTileN + 1;
+  return run_form<b200::kFormTree>(f, w, max_tiles, sms, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -68,11 +68,23 @@
 //                are masked; their mask bits are gathered by ballots, one
 //                coalesced read of the mask row per query position.
 // Both keep every index inside the caller's sizes (rows, mask columns, work
-// list), whatever the device-side lengths say, and hold the partial O of split
-// units in fp32.
-// Registers: launched at 168 per thread (the 384-thread limit); the first
-// warpgroup gives back down to 104 and the softmax warpgroups take 200 each
-// (104 + 2 x 200 = 3 x 168, the launch's total).
+// list), whatever the device-side lengths say.  kFormPrompt takes its units from
+// the schedule kernel's list; kFormPromptStream (small batches) and kFormTree
+// differ from it in two things, because launches, balance and the latency of one
+// tile's softmax decide there:
+//   * no schedule kernel.  Every unit counts ticks: an overhead, and per KV tile
+//     one (a single query tile) or two (two of them).  CTA i of C takes the i-th
+//     C-th of all ticks, which it finds from the lengths by one block scan.  A
+//     CTA's first and last unit may be pieces of units that it shares with its
+//     neighbours: their fp32 partials (O, m, l) go to slots 2 i and 2 i + 1 and
+//     stream_combine_kernel joins them.
+//   * single-tile units (at most P positions; not at head_dim 256, whose O fills
+//     the TMEM): both softmax warpgroups work on the one query tile, warpgroup t on
+//     the KV tiles j = t (mod 2) with S_t, O_t, m, l of its own, so a tile's softmax
+//     latency hides behind the other's (64 sequences x 12K keys, 8 rows each: 232 ->
+//     164 us).  At the end warpgroup 0 turns both m, l into the weights of O_0 and
+//     O_1, and each warpgroup joins and stores half of the columns from TMEM (both O
+//     lie in the same lanes).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -104,7 +116,8 @@ constexpr float kRescaleSum = 256.0f;      // 2^kRescaleThreshold
 constexpr uint32_t kSmQ = 0;                            // Q0, Q1: 2 x (2 x 16 KB)
 constexpr uint32_t kSmKV = 65536;                       // ring: kKvStages x 32 KB
 constexpr uint32_t kSmBar = kSmKV + kKvStages * 32768;  // mbarriers, TMEM slot, abort flag, unit ring
-constexpr uint32_t kSmBytes = kSmBar + 512;
+constexpr uint32_t kSmMl = kSmBar + 512;                // 128 x (m, l) of warpgroup 1 (bounded forms)
+constexpr uint32_t kSmBytes = kSmMl + 1024;
 constexpr uint32_t kAttnSmemAlloc = kSmBytes + 1024;    // + alignment slack
 static_assert(kAttnSmemAlloc <= 232448, "shared memory per CTA");
 constexpr int kUnitRing = 4;  // claimed work units in flight between the producer and the consumers
@@ -120,18 +133,25 @@ enum : int {
   BAR_IT_FULL = BAR_O_DONE + 2,              // + ring entry
   BAR_IT_EMPTY = BAR_IT_FULL + kUnitRing,    // + ring entry
   BAR_DRAIN = BAR_IT_EMPTY + kUnitRing,
-  BAR_COUNT = BAR_DRAIN + 1
+  BAR_ML_FULL = BAR_DRAIN + 1,               // single-tile unit: warpgroup 1's m, l are there
+  BAR_ML_JOIN = BAR_ML_FULL + 1,             // warpgroup 0 has turned them into the weights of O_0, O_1
+  BAR_ML_DONE = BAR_ML_JOIN + 1,             // both have read O_0 and O_1
+  BAR_COUNT = BAR_ML_DONE + 1
 };
 
 // A claimed unit as the producer publishes it: (seq, qunit, kvh, split, the
 // unit's split count, its partial-output slot), then cu_q[seq], cu_q[seq + 1],
 // seqused[seq] and a valid flag (0 ends the loop).
-// kFormPrompt also carries the first K/V row of the sequence.
+// kFormPrompt also carries the first K/V row of the sequence.  The bounded forms
+// hold the piece's first KV tile in split, the tile behind its last in nsplit, and
+// in slot its partial slot (-1: the whole unit).
 struct UnitEntry {
   int seq, qunit, kvh, split, nsplit, slot, q_begin, q_end, seq_len, valid, k_begin;
 };
 
-enum : int { kFormPaged = 0, kFormPrompt = 1, kFormTree = 2 };
+enum : int { kFormPaged = 0, kFormPrompt = 1, kFormPromptStream = 2, kFormTree = 3 };
+constexpr bool form_rows(int form) { return form == kFormPrompt || form == kFormPromptStream; }  // plain K/V rows
+constexpr bool form_streamed(int form) { return form == kFormPromptStream || form == kFormTree; }
 
 // Work-list entry: x = sequence, y = query unit, z = KV head | split << 16 |
 // split count << 24, w = partial-output slot of a split unit (-1 unsplit).
@@ -146,6 +166,7 @@ __device__ __forceinline__ void unpack_unit(const int4 u, int& kvh, int& split, 
 constexpr int kUnitRows = 256;  // partial rows per split unit: 2 query tiles x 128 rows
 constexpr uint32_t kSmRing = BAR_COUNT * 8 + 16;  // after the barriers, the TMEM slot and the abort flag
 static_assert(kSmRing + kUnitRing * sizeof(UnitEntry) <= 512, "barrier area");
+static_assert(kSmRing % 8 == 0 && kUnitRing * sizeof(UnitEntry) >= kAttnThreads / 32 * 8 + 6 * 4, "scratch of stream_share");
 
 struct AttnKernelArgs {
   const void* block_table;
@@ -178,6 +199,9 @@ struct AttnKernelArgs {
   int mask_cols;
   int total_k;
   int full;                  // every row's keys end at L (bidirectional, or masked by the tree)
+  int wide_out;              // rows of out are 32-byte aligned
+  int num_seqs, num_kv_heads;
+  int4* stream_meta;         // [grid]: sequence, query unit, KV head, pieces of the unit that CTA i begins and does not end (0: none)
 };
 
 // K/V tensor maps.  Up to kMaxHeadMaps KV heads: one 5-D map per head,
@@ -228,7 +252,7 @@ __device__ __forceinline__ SeqBounds seq_bounds(const Args& a, int b) {
     s.q_begin = min(max(s.q_begin, 0), a.total_q);
     s.q_end = min(max(s.q_end, s.q_begin), a.total_q);
   }
-  if (kForm == kFormPrompt) {
+  if (form_rows(kForm)) {
     s.k_begin = min(max(load_index(a.cu_k, b, a.len_i64), 0), a.total_k);
     s.seq_len = min(max(load_index(a.cu_k, b + 1, a.len_i64), s.k_begin), a.total_k) - s.k_begin;
   } else {
@@ -268,6 +292,164 @@ __device__ __forceinline__ UnitGeom unit_geometry(int q_begin, int q_end, int se
   u.kv_lo = u.split_begin;
   u.n_tiles = (u.kv_hi > u.split_begin) ? (u.kv_hi - u.kv_lo + kAttnTileN - 1) / kAttnTileN : 0;
   return u;
+}
+
+// A piece of a unit in the bounded forms: KV tiles [tile_lo, tile_hi).
+__device__ __forceinline__ UnitGeom piece_geometry(int q_begin, int q_end, int seq_len, int qunit, int tile_lo,
+                                                   int tile_hi, int pos_per_unit, int full) {
+  UnitGeom u;
+  u.q_begin = q_begin;
+  u.q_len = q_end - q_begin;
+  u.seq_len = seq_len;
+  u.pos0 = qunit * pos_per_unit;
+  const int rows = min(pos_per_unit, u.q_len - u.pos0);
+  u.q_abs_min = seq_len - u.q_len + u.pos0;
+  const int kv_end = full ? max(seq_len, 0) : max(min(max(seq_len, 0), u.q_abs_min + rows), 0);
+  u.kv_lo = u.split_begin = tile_lo * kAttnTileN;
+  u.kv_hi = u.split_end = min(tile_hi * kAttnTileN, kv_end);
+  u.n_tiles = tile_hi - tile_lo;
+  return u;
+}
+
+// Streamed work.  Ticks of a unit: kStreamOverhead + k tiles, k = 2 where two query
+// tiles share the KV tiles, else 1 (a tick is about a microsecond).
+constexpr int kStreamOverhead = 2;
+constexpr int kStreamMinTicks = 3;  // a CTA's share at least
+constexpr int kStreamMinTiles = 2;  // KV tiles of a piece at least: fewer do not pay for its partial
+
+__device__ __forceinline__ int unit_weight(bool wide, int q_len, int qunit, int pos_per_unit) {
+  return !wide && q_len - qunit * pos_per_unit > pos_per_unit / 2 ? 2 : 1;
+}
+
+// Ticks of one sequence: its query units, each for every KV head.
+template <int kForm, bool kWide>
+__device__ __forceinline__ long long seq_ticks(const AttnKernelArgs& a, const SeqBounds& sb, int ppu) {
+  const int q_len = sb.q_end - sb.q_begin;
+  if (q_len <= 0) return 0;
+  const int nq = (q_len + ppu - 1) / ppu;
+  long long t = 0;
+  if (kForm == kFormTree || a.full) {
+    const int tiles = (sb.seq_len + kAttnTileN - 1) / kAttnTileN;
+    t = static_cast<long long>(nq) * kStreamOverhead +
+        static_cast<long long>(tiles) * ((nq - 1) * (kWide ? 1 : 2) + unit_weight(kWide, q_len, nq - 1, ppu));
+  } else {
+    for (int q = 0; q < nq; ++q)
+      t += kStreamOverhead + unit_weight(kWide, q_len, q, ppu) * qunit_full_tiles(q_len, sb.seq_len, q, ppu);
+  }
+  return t * a.num_kv_heads;
+}
+
+// The unit in which tick x lies, given its sequence and that one's first tick.
+struct StreamUnit {
+  int first, weight, tiles, qunit, kvh;
+  __device__ __forceinline__ int ticks() const { return kStreamOverhead + weight * tiles; }
+};
+template <int kForm, bool kWide>
+__device__ __forceinline__ StreamUnit stream_unit(const AttnKernelArgs& a, const SeqBounds& sb, int seq_first, int x,
+                                                  int ppu) {
+  const int q_len = sb.q_end - sb.q_begin;
+  const int nq = (q_len + ppu - 1) / ppu;
+  StreamUnit u;
+  u.first = seq_first;
+  u.qunit = 0;
+  if (kForm == kFormTree || a.full) {
+    u.tiles = (sb.seq_len + kAttnTileN - 1) / kAttnTileN;
+    if (nq > 1) {  // every query unit but the last has the same ticks
+      const int row = (kStreamOverhead + (kWide ? 1 : 2) * u.tiles) * a.num_kv_heads;
+      u.qunit = min((x - seq_first) / row, nq - 1);
+      u.first += u.qunit * row;
+    }
+    u.weight = unit_weight(kWide, q_len, u.qunit, ppu);
+  } else {
+    for (;; ++u.qunit) {
+      u.tiles = qunit_full_tiles(q_len, sb.seq_len, u.qunit, ppu);
+      u.weight = unit_weight(kWide, q_len, u.qunit, ppu);
+      const int row = u.ticks() * a.num_kv_heads;
+      if (x < u.first + row || u.qunit + 1 >= nq) break;
+      u.first += row;
+    }
+  }
+  u.kvh = min((x - u.first) / u.ticks(), a.num_kv_heads - 1);
+  u.first += u.kvh * u.ticks();
+  return u;
+}
+
+// A share ends at a tile of the unit in which its raw tick falls, or at the unit's
+// start or end where fewer than kStreamMinTiles tiles would be left on that side.
+__device__ __forceinline__ int stream_snap(const StreamUnit& u, int x) {
+  const int tile = (x - u.first - kStreamOverhead) / u.weight;
+  if (x - u.first < kStreamOverhead || tile < kStreamMinTiles) return u.first;
+  if (u.tiles - tile < kStreamMinTiles) return u.first + u.ticks();
+  return u.first + kStreamOverhead + tile * u.weight;
+}
+
+// A CTA's share: ticks [x, end), x in (or at the end of) sequence seq, whose first
+// tick is seq_first; of ctas shares in all, share i begins near tick raw(i).
+struct StreamShare {
+  int x, end, seq, seq_first;
+  int base, extra, ctas;
+  __device__ __forceinline__ int raw(int i) const { return i * base + min(i, extra); }
+};
+
+// Block-wide; scratch: 12 long longs and 6 ints of shared memory.  `mine`: the
+// bounds of sequence threadIdx.x (loaded early), if there is one.
+template <int kForm, bool kWide>
+__device__ __forceinline__ StreamShare stream_share(const AttnKernelArgs& a, const SeqBounds& mine, int ppu,
+                                                    long long* scratch) {
+  const int per = (a.num_seqs + kAttnThreads - 1) / kAttnThreads;
+  const int s0 = min(static_cast<int>(threadIdx.x) * per, a.num_seqs), s1 = min(s0 + per, a.num_seqs);
+  long long ticks = 0;
+  for (int b = s0; b < s1; ++b) ticks += seq_ticks<kForm, kWide>(a, per == 1 ? mine : seq_bounds<kForm>(a, b), ppu);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long sum = ticks;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
+  }
+  if (lane == 31) scratch[warp] = sum;
+  __syncthreads();
+  long long before = sum - ticks, all = 0;
+#pragma unroll
+  for (int w = 0; w < kAttnThreads / 32; ++w) {
+    if (w < warp) before += scratch[w];
+    all += scratch[w];
+  }
+  // The host has bounded the ticks of sequences that do not overlap; of others the rest is dropped.
+  const int total = static_cast<int>(min(all, 0x7fffffffll));
+  StreamShare sh;
+  sh.ctas = max(1, min(static_cast<int>(gridDim.x), total / kStreamMinTicks));
+  sh.base = total / sh.ctas;
+  sh.extra = total - sh.base * sh.ctas;
+  int* out = reinterpret_cast<int*>(scratch + kAttnThreads / 32);  // (snapped tick, sequence, its first tick) of both ends
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int at = sh.raw(min(static_cast<int>(blockIdx.x) + k, sh.ctas));
+    if (threadIdx.x == 0 && at >= total) {
+      out[3 * k] = total;
+      out[3 * k + 1] = a.num_seqs;
+      out[3 * k + 2] = total;
+    }
+    if (at < total && at >= before && at < before + ticks) {
+      long long first = before;
+      int b = s0;
+      SeqBounds sb = per == 1 ? mine : seq_bounds<kForm>(a, b);
+      for (; b + 1 < s1; sb = seq_bounds<kForm>(a, ++b)) {
+        const long long t = seq_ticks<kForm, kWide>(a, sb, ppu);
+        if (at < first + t) break;
+        first += t;
+      }
+      out[3 * k] = stream_snap(stream_unit<kForm, kWide>(a, sb, static_cast<int>(first), at, ppu), at);
+      out[3 * k + 1] = b;
+      out[3 * k + 2] = static_cast<int>(first);
+    }
+  }
+  __syncthreads();
+  sh.x = out[0];
+  sh.seq = out[1];
+  sh.seq_first = out[2];
+  sh.end = out[3];
+  return sh;
 }
 
 template <typename T>
@@ -317,7 +499,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kTilesPerUnit = kWide ? 1 : kAttnTilesPerUnit;
   constexpr int kFillsPerTile = kWide ? 4 : 2;  // ring slots per KV tile: K (, K hi), V (, V hi)
-  static_assert(kForm != kFormPrompt || !kHeadMaps, "plain rows use one map for all heads");
+  static_assert(!form_rows(kForm) || !kHeadMaps, "plain rows use one map for all heads");
+  constexpr bool kStreamed = form_streamed(kForm);
   griddep_wait();  // launched as a programmatic dependent of the schedule kernel
 
   extern __shared__ uint8_t smem_raw[];
@@ -333,6 +516,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int lane = threadIdx.x % 32;
   const int P = a.pos_per_tile;
   const int ppu = kTilesPerUnit * P;
+  SeqBounds my_seq{};  // streamed work: loaded here, used after the set-up
+  if (kStreamed && static_cast<int>(threadIdx.x) < a.num_seqs) my_seq = seq_bounds<kForm>(a, threadIdx.x);
 
   if (threadIdx.x == 0) {
     mbar_init(bar(BAR_Q_FULL), 1);
@@ -351,6 +536,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(bar(BAR_IT_EMPTY + r), 9);  // the MMA issuer and the 8 softmax warps
     }
     mbar_init(bar(BAR_DRAIN), 1);
+    if (kStreamed) {
+      mbar_init(bar(BAR_ML_FULL), 4);
+      mbar_init(bar(BAR_ML_JOIN), 4);
+      mbar_init(bar(BAR_ML_DONE), 8);
+    }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -370,6 +560,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     fence_proxy_async_smem();
   }
+  // Streamed work: this CTA's share (the unit ring's memory serves as scratch).
+  StreamShare share{};
+  if (kStreamed)
+    share = stream_share<kForm, kWide>(a, my_seq, ppu, reinterpret_cast<long long*>(smem + kSmBar + kSmRing));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -393,9 +587,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     return true;
   };
   auto geometry = [&](const UnitEntry& e) {
-    return unit_geometry(e.q_begin, e.q_end, e.seq_len, e.qunit, e.split, e.nsplit, ppu,
-                         kForm == kFormPaged ? 0 : kForm == kFormTree ? 1 : a.full);
+    if (kForm != kFormPaged)
+      return piece_geometry(e.q_begin, e.q_end, e.seq_len, e.qunit, e.split, e.nsplit, ppu,
+                            kForm == kFormTree ? 1 : a.full);
+    return unit_geometry(e.q_begin, e.q_end, e.seq_len, e.qunit, e.split, e.nsplit, ppu);
   };
+  // Both warpgroups on one query tile (see the header comment).
+  auto is_dual = [&](const UnitGeom& ug) { return kStreamed && !kWide && ug.pos0 + P >= ug.q_len; };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAttnProducerRegs));
@@ -406,16 +604,60 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tma_prefetch_desc(&maps.k[lane]);
         tma_prefetch_desc(&maps.v[lane]);
       }
-      const int unit_count = *a.unit_count;
+      const int unit_count = kStreamed ? 0 : *a.unit_count;
       int* claim = const_cast<int*>(a.unit_count) + 1;  // reset to 0 by the schedule kernel
       int issued = 0;   // K/V ring fills so far
       int q_loads = 0;  // Q loads so far
       const int my_slice = lane & 7;
+      int4 meta = make_int4(0, 0, 0, 0);
+      if (kStreamed && lane == 0) a.stream_meta[blockIdx.x] = meta;  // also when the loop below gives up early
+      if (kStreamed && static_cast<int>(blockIdx.x) >= share.ctas) share.end = share.x;
       for (int it = 0;; ++it) {
+        UnitEntry e{};
+        if (kStreamed) {
+          e.valid = share.x < share.end;
+          while (e.valid) {
+            const SeqBounds sb = seq_bounds<kForm>(a, share.seq);
+            const long long ticks = seq_ticks<kForm, kWide>(a, sb, ppu);
+            if (share.x >= share.seq_first + ticks) {  // the sequence's units are done (or it has none)
+              share.seq_first += static_cast<int>(ticks);
+              if (++share.seq >= a.num_seqs) e.valid = 0;
+              continue;
+            }
+            const StreamUnit u = stream_unit<kForm, kWide>(a, sb, share.seq_first, share.x, ppu);
+            const int unit_end = u.first + u.ticks();
+            const int piece_end = min(share.end, unit_end);
+            const bool from_start = share.x == u.first, to_end = piece_end == unit_end;
+            e.seq = share.seq;
+            e.qunit = u.qunit;
+            e.kvh = u.kvh;
+            // Shares end on tiles: dividing by a weight of 1 or 2 is exact.
+            e.split = from_start ? 0 : (share.x - u.first - kStreamOverhead) >> (u.weight - 1);
+            e.nsplit = to_end ? u.tiles : (piece_end - u.first - kStreamOverhead) >> (u.weight - 1);
+            e.slot = from_start && to_end ? -1 : 2 * static_cast<int>(blockIdx.x) + (from_start ? 1 : 0);
+            e.q_begin = sb.q_begin;
+            e.q_end = sb.q_end;
+            e.seq_len = sb.seq_len;
+            e.k_begin = sb.k_begin;
+            if (from_start && !to_end) {
+              // The CTAs behind this one whose share begins inside the unit hold its other pieces.
+              int pieces = 1;
+              for (int i0 = static_cast<int>(blockIdx.x) + 1; i0 < share.ctas; i0 += 32) {
+                const int i = i0 + lane, x = i < share.ctas ? share.raw(i) : unit_end;
+                const unsigned in = __ballot_sync(0xffffffffu, x < unit_end && stream_snap(u, x) < unit_end);
+                pieces += __popc(in);
+                if (in != 0xffffffffu) break;
+              }
+              meta = make_int4(e.seq, e.qunit, e.kvh, pieces);
+            }
+            share.x = piece_end;
+            break;
+          }
+          if (!e.valid && lane == 0) a.stream_meta[blockIdx.x] = meta;
+        } else {
         int u = 0;
         if (lane == 0) u = atomicAdd(claim, 1);
         u = __shfl_sync(0xffffffffu, u, 0);
-        UnitEntry e{};
         e.valid = u < unit_count;
         if (e.valid) {
           const int4 un = a.units[u];
@@ -428,6 +670,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           e.q_end = sb.q_end;
           e.seq_len = sb.seq_len;
           e.k_begin = sb.k_begin;
+          if (kForm != kFormPaged) {  // whole units
+            e.split = 0;
+            e.nsplit = qunit_full_tiles(e.q_end - e.q_begin, e.seq_len, e.qunit, ppu, kForm == kFormTree ? 1 : a.full);
+            e.slot = -1;
+          }
+        }
         }
         int ok = 1;
         if (lane == 0) {
@@ -488,28 +736,40 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const int v = load_index(a.block_table, bt_row + lpc, a.bt_i64);
           pg = (pos < ug.kv_hi && lp < a.bt_cols) ? v : a.num_blocks;
         };
-        int pg_cur = 0, of_cur = 0, pg_nxt = a.num_blocks, of_nxt = 0;
-        if (kForm != kFormPrompt) {
+        int pg_cur = 0, of_cur = 0, pg_nxt = a.num_blocks, of_nxt = 0, pg_prev = 0, of_prev = 0;
+        if (!form_rows(kForm)) {
           lookup(0, pg_cur, of_cur);
           if (n_tiles > 1) lookup(1, pg_nxt, of_nxt);
         }
         bool stop = false;
+        const bool dual = is_dual(ug);
         for (int idx = 0; idx < kFillsPerTile * n_tiles; ++idx) {
-          const int j = idx / kFillsPerTile;
-          const int part = idx % kFillsPerTile;  // K, V  or  K lo, K hi, V lo, V hi
+          int j = idx / kFillsPerTile;
+          int part = idx % kFillsPerTile;  // K, V  or  K lo, K hi, V lo, V hi
+          if (dual) {  // K0, K1, V0, K2, V1, ..: the order in which the UMMAs need them
+            part = idx > 1 && (idx % 2 == 0 || idx + 1 == 2 * n_tiles);
+            if (n_tiles == 1) part = idx;
+            j = part ? (idx + 1 == 2 * n_tiles ? n_tiles - 1 : idx / 2 - 1) : (idx + 1) / 2;
+          }
           const bool is_v = part >= kFillsPerTile / 2;
           const int hi = kWide ? (part & 1) : 0;  // 128-column half of a head_dim-256 row
           const int slot = issued % kKvStages;
           const uint32_t ph = (issued / kKvStages) & 1;
-          if (kForm != kFormPrompt && part == 0 && j > 0) {
+          if (!form_rows(kForm) && part == 0 && j > 0) {
+            if (kForm == kFormTree) {
+              pg_prev = pg_cur;
+              of_prev = of_cur;
+            }
             pg_cur = pg_nxt;
             of_cur = of_nxt;
             if (j + 1 < n_tiles) lookup(j + 1, pg_nxt, of_nxt);
           }
           // 4-D maps: lanes 0..15 issue half lane & 1 of slice (lane >> 1); head_dim 64: lane c < 8 slice c.
           const int c = kNarrow ? (lane & 7) : ((lane >> 1) & 7);
-          const int page = kHeadMaps ? pg_cur : __shfl_sync(0xffffffffu, pg_cur, c);
-          const int off = kHeadMaps ? of_cur : __shfl_sync(0xffffffffu, of_cur, c);
+          const bool behind = dual && is_v && j + 1 < n_tiles;  // V_j comes after K_{j + 1}
+          const int pg = behind ? pg_prev : pg_cur, of = behind ? of_prev : of_cur;
+          const int page = kHeadMaps ? pg : __shfl_sync(0xffffffffu, pg, c);
+          const int off = kHeadMaps ? of : __shfl_sync(0xffffffffu, of, c);
           if (lane == 0) {
             ok = mbar_wait(bar(BAR_KV_EMPTY + slot), ph ^ 1, abort_flag);
             if (ok) mbar_arrive_expect_tx(bar(BAR_KV_FULL + slot), kNarrow ? 16384 : 32768);
@@ -518,7 +778,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             stop = true;
             break;
           }
-          if (kForm == kFormPrompt) {
+          if (form_rows(kForm)) {
             // 128 rows x 64 columns a copy (16 KB), one per half; rows past the tensor are zero fill.
             if (lane < (kNarrow ? 1 : 2))
               tma_load_3d(sbase + kSmKV + slot * 32768 + lane * 16384, is_v ? &maps.v[0] : &maps.k[0],
@@ -564,8 +824,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // address field (shared addresses stay below 256 KB, so the 14-bit field
       // never carries).  Every instruction between two UMMAs idles the tensor
       // core, which takes only about one UMMA ahead of execution.
-      auto issue_s = [&](int t, uint32_t kslot_addr) {
-        const uint64_t qd = umma_desc_sw128(sbase + kSmQ + t * 32768, 16, 1024);
+      auto issue_s = [&](int t, uint32_t kslot_addr, int q_tile) {
+        const uint64_t qd = umma_desc_sw128(sbase + kSmQ + q_tile * 32768, 16, 1024);
         const uint64_t kd = umma_desc_sw128(kslot_addr, 16, kKvSbo);
 #pragma unroll
         for (int kk = 0; kk < kQkSteps; ++kk) {
@@ -675,11 +935,44 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const int n_tiles = ug.n_tiles;
         if (n_tiles == 0) continue;
         const bool two = ug.pos0 + P < ug.q_len;
+        if (is_dual(ug)) {
+          // Tile j on S_t, O_t with t = j mod 2; the query tile is the same.
+          bool go = mbar_wait(bar(BAR_Q_FULL), q_uses & 1, abort_flag);
+          for (int j = 0; go && j < min(n_tiles, 2); ++j) {
+            go = wait_full(fills + j);
+            if (!go) break;
+            tc_fence_after();
+            issue_s(j, slot_addr(fills + j), 0);
+            if (j + 1 == n_tiles) tc_commit(bar(BAR_Q_EMPTY));
+            tc_commit(bar(BAR_KV_EMPTY + (fills + j) % kKvStages));
+          }
+          for (int j = 0; go && j < n_tiles; ++j) {
+            const int t = j & 1, vidx = fills + (j + 1 == n_tiles ? 2 * n_tiles - 1 : 2 * j + 2);
+            go = wait_full(vidx) && issue_pv(t, tiles_done[t] + (j >> 1), slot_addr(vidx), j > 1, j + 2 >= n_tiles);
+            if (!go) break;
+            tc_commit(bar(BAR_KV_EMPTY + vidx % kKvStages));
+            if (j + 2 < n_tiles) {
+              const int kidx = fills + 2 * j + 3;
+              go = wait_full(kidx);
+              if (!go) break;
+              tc_fence_after();
+              issue_s(t, slot_addr(kidx), 0);
+              if (j + 3 == n_tiles) tc_commit(bar(BAR_Q_EMPTY));
+              tc_commit(bar(BAR_KV_EMPTY + kidx % kKvStages));
+            }
+          }
+          if (!go) break;
+          fills += 2 * n_tiles;
+          ++q_uses;
+          tiles_done[0] += (n_tiles + 1) / 2;
+          tiles_done[1] += n_tiles / 2;
+          continue;
+        }
         bool ok = mbar_wait(bar(BAR_Q_FULL), q_uses & 1, abort_flag) && wait_full(fills);
         if (ok) {
           tc_fence_after();
-          issue_s(0, slot_addr(fills));
-          if (two) issue_s(1, slot_addr(fills));
+          issue_s(0, slot_addr(fills), 0);
+          if (two) issue_s(1, slot_addr(fills), 1);
           if (n_tiles == 1) tc_commit(bar(BAR_Q_EMPTY));
           tc_commit(bar(BAR_KV_EMPTY + fills % kKvStages));
         }
@@ -696,14 +989,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               break;
             }
             tc_fence_after();
-            issue_s(0, slot_addr(kidx));
+            issue_s(0, slot_addr(kidx), 0);
           }
           if (two) {
             if (!issue_pv(1, tiles_done[1] + j, slot_addr(vidx), j > 0, !more)) {
               ok = false;
               break;
             }
-            if (more) issue_s(1, slot_addr(kidx));
+            if (more) issue_s(1, slot_addr(kidx), 1);
           }
           if (more && j + 2 == n_tiles) tc_commit(bar(BAR_Q_EMPTY));  // the unit's last S is issued
           tc_commit(bar(BAR_KV_EMPTY + vidx % kKvStages));
@@ -732,7 +1025,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     int fills = 0;       // K/V ring fills of the units before this one
     int tiles_done = 0;  // tiles this group processed in earlier units
     int o_units = 0;     // O_DONE phases seen: one per unit with tiles for this group
+    int o_units_other = 0;   // the same of the other group (streamed work)
+    int joins = 0;           // single-tile units so far: phases of ML_FULL / ML_JOIN / ML_DONE
+    bool join_open = false;  // the other group may still read this group's O of the last one
     bool aborted = false;
+    auto warp_wait = [&](int b, int phase) {  // one answer for the warp, which stays together
+      return __all_sync(0xffffffffu, mbar_wait(bar(b), phase & 1, abort_flag)) != 0;
+    };
     for (int it = 0; !aborted; ++it) {
       UnitEntry e;
       if (!take_entry(it, e)) break;
@@ -744,29 +1043,36 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const bool two = !kWide && ug.pos0 + P < ug.q_len;
       const int unit_fills = fills;
       fills += kFillsPerTile * n_tiles;
-      if (!(t == 0 || two)) continue;
-      const int tile_pos0 = ug.pos0 + t * P;
+      const bool dual = is_dual(ug) && n_tiles > 0;
+      if (!(t == 0 || two || dual)) continue;
+      const int q_tile = dual ? 0 : t;         // query tile of this group
+      const int step = dual ? 2 : 1;           // its KV tiles: first_j, first_j + step, ..
+      const int first_j = dual ? t : 0;
+      const int own = dual ? (n_tiles + 1 - t) >> 1 : n_tiles;
+      const int last_t = kStreamed && dual ? (n_tiles - 1) & 1 : 0;  // the group that clears V's tail
+      const int tile_pos0 = ug.pos0 + q_tile * P;
       const int row_pos = tile_pos0 + row / a.group;
       const int row_head = e.kvh * a.group + row % a.group;
       const bool row_valid = row < q_rows && row_pos < ug.q_len;
-      const int q_abs = ug.q_abs_min + t * P + row / a.group;
-      const bool full = kForm == kFormPrompt && a.full;
+      const int q_abs = ug.q_abs_min + q_tile * P + row / a.group;
+      const bool full = form_rows(kForm) && a.full;
       const int row_hi = (kForm == kFormTree || full) ? ug.split_end : min(ug.split_end, q_abs + 1);
       const int ctx = ug.seq_len - ug.q_len;  // kFormTree: keys at or past it are drafted tokens
       const int unmasked_hi = kForm == kFormTree ? min(ug.split_end, ctx)
                               : full             ? ug.split_end
-                                                 : min(ug.split_end, ug.q_abs_min + t * P + 1);
+                                                 : min(ug.split_end, ug.q_abs_min + q_tile * P + 1);
       // V rows [v_tail_from, v_tail_to) of the last tile: loaded page rows at or past L.
       const int last_start = ug.kv_lo + (n_tiles - 1) * kAttnTileN;
       const int v_tail_from = max(ug.seq_len - last_start, 0);
-      const int v_tail_to = kForm == kFormPrompt
+      const int v_tail_to = form_rows(kForm)
                                 ? kAttnTileN
                                 : min(((ug.kv_hi + kAttnSlice - 1) / kAttnSlice) * kAttnSlice - last_start, kAttnTileN);
 
       float m_used = -INFINITY;  // running maximum in scaled base-2 units
       float l = 0.f;
-      for (int j = 0; j < n_tiles; ++j) {
-        const int c = tiles_done + j;
+      for (int jj = 0; jj < own; ++jj) {
+        const int j = first_j + jj * step;
+        const int c = tiles_done + jj;
         if (!mbar_wait(bar(BAR_S_FULL + t), c & 1, abort_flag)) {
           aborted = true;
           break;
@@ -874,7 +1180,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const bool raise = m_cand > m_used + kRescaleThreshold;  // false while both are -inf
         if (__any_sync(0xffffffffu, raise)) {
           const float alpha = raise ? ex2_approx(m_used - m_cand) : 1.f;  // 0 when m_used = -inf
-          if (j > 0) {
+          if (jj > 0) {
             // O holds PV of tiles < j: scale it before PV_j accumulates.  The
             // S_FULL phase of tile j already implies PV_{j-1} is complete: its
             // commit covers every UMMA the issuer started before S_j.
@@ -895,13 +1201,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
         }  // !fast
         const float neg_m = (m_used == -INFINITY) ? 0.f : -m_used;
-        if (t == 0 && j == n_tiles - 1 && v_tail_from < v_tail_to) {
+        if (t == last_t && j == n_tiles - 1 && v_tail_from < v_tail_to) {
           // Rows of the last page past the sequence end may hold anything (NaN
           // included); P is 0 there but 0 * NaN is NaN, so zero those V rows,
           // as the reference's masked V load does (triton_split_kv_paged.py:122).
           bool landed = true;
           for (int vs = 0; vs < (kWide ? 2 : 1) && landed; ++vs) {  // the V slot(s) of the last tile
-            const int vidx = unit_fills + kFillsPerTile * j + kFillsPerTile / 2 + vs;
+            const int vidx = unit_fills + kFillsPerTile * j + kFillsPerTile / 2 + vs;  // the unit's last fill(s)
             if (!mbar_wait(bar(BAR_KV_FULL + vidx % kKvStages), (vidx / kKvStages) & 1, abort_flag)) {
               landed = false;
               break;
@@ -909,7 +1215,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             const uint32_t vbase = sbase + kSmKV + (vidx % kKvStages) * 32768;
             constexpr int kHalves = kNarrow ? 1 : 2;  // 64-column halves per row in a slot
             const int n16 = (v_tail_to - v_tail_from) * 8 * kHalves;  // 16-byte pieces
-            for (int i = threadIdx.x - 128; i < n16; i += 128) {
+            for (int i = threadIdx.x - 128 - 128 * last_t; i < n16; i += 128) {
               const int r = v_tail_from + i / (8 * kHalves);
               const int half = (i >> 3) & (kHalves - 1);
               st_shared_v4(vbase + kv_slot_offset<kHeadMaps, kNarrow>(r, half, i & 7), 0u, 0u, 0u, 0u);
@@ -938,6 +1244,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
           tmem_st16(s_addr + 16 * c4, pk);
           }
+          if (kStreamed && c4 == 1 && join_open) {
+            // The first P of this unit lets P V overwrite O_t: the other group has read the last one first.
+            join_open = false;
+            if (!warp_wait(BAR_ML_DONE, joins - 1)) aborted = true;
+          }
           if (c4 % 2 == 1) {  // publish P in halves: two waits for the issuer per tile instead of four
             tmem_wait_st();
             tc_fence_before();
@@ -953,24 +1264,73 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
 
       // ---------------------------------------------------------- epilogue
-      if (!aborted && n_tiles > 0) {
-        if (!mbar_wait(bar(BAR_O_DONE + t), o_units & 1, abort_flag)) aborted = true;
+      if (kStreamed) aborted = __any_sync(0xffffffffu, aborted);
+      if (!aborted && own > 0) {
+        if (!(kStreamed ? warp_wait(BAR_O_DONE + t, o_units) : mbar_wait(bar(BAR_O_DONE + t), o_units & 1, abort_flag)))
+          aborted = true;
         tc_fence_after();
         ++o_units;
       }
-      tiles_done += n_tiles;
+      tiles_done += own;
       if (aborted) break;
-      const float inv = 1.f / fmaxf(l, 1e-20f);
+      const float inv_self = 1.f / fmaxf(l, 1e-20f);
+      float w_self = inv_self, w_other = 0.f;  // weights of this group's O and, in a single-tile unit, of the other's
+      const bool join = kStreamed && dual && n_tiles > 1;  // both groups have an O
+      if (kStreamed && !dual && two && n_tiles > 0) ++o_units_other;
+      if (kStreamed && dual) {
+        volatile float* ml = reinterpret_cast<volatile float*>(smem + kSmMl) + 2 * row;
+        // O of both groups is complete: own > 0 waited for this group's above.
+        if (n_tiles > 1 || t == 1) {
+          if (!warp_wait(BAR_O_DONE + (t ^ 1), o_units_other)) aborted = true;
+          ++o_units_other;
+        }
+        if (join_open && !aborted) {  // only if no P was published since: the last unit's weights are read
+          if (!warp_wait(BAR_ML_DONE, joins - 1)) aborted = true;
+        }
+        if (t == 1 && !aborted) {
+          ml[0] = m_used;
+          ml[1] = l;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(BAR_ML_FULL));
+          if (!warp_wait(BAR_ML_JOIN, joins)) aborted = true;
+          w_other = ml[0];  // of O_0
+          w_self = ml[1];
+        } else if (!aborted) {
+          if (!warp_wait(BAR_ML_FULL, joins)) aborted = true;
+          const float m1 = ml[0], l1 = ml[1];
+          const float m_all = fmaxf(m_used, m1);
+          const float s0 = m_used == -INFINITY ? 0.f : ex2_approx(m_used - m_all);
+          const float s1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - m_all);
+          l = l * s0 + (s1 != 0.f ? l1 * s1 : 0.f);
+          m_used = m_all;
+          const float inv = 1.f / fmaxf(l, 1e-20f);
+          w_self = s0 * inv;
+          w_other = s1 * inv;
+          ml[0] = w_self;
+          ml[1] = w_other;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(BAR_ML_JOIN));
+        }
+        if (aborted) break;
+        __syncwarp();
+        tc_fence_after();
+        ++joins;
+        join_open = true;
+      }
       const int tok = ug.q_begin + row_pos;
       T* dst = nullptr;
       float* dst32 = nullptr;  // partial O of the bounded forms
-      if (e.nsplit <= 1) {
+      if (kForm != kFormPaged ? e.slot < 0 : e.nsplit <= 1) {
         dst = static_cast<T*>(a.out) + static_cast<int64_t>(tok) * a.out_st + static_cast<int64_t>(row_head) * a.out_sh;
       } else {
-        const int64_t rowi = (static_cast<int64_t>(e.slot) * a.num_splits + e.split) * kUnitRows + t * kAttnTileM + row;
+        const int64_t rowi = kForm != kFormPaged
+                                 ? static_cast<int64_t>(e.slot) * kUnitRows + q_tile * kAttnTileM + row
+                                 : (static_cast<int64_t>(e.slot) * a.num_splits + e.split) * kUnitRows + t * kAttnTileM + row;
         if (kForm == kFormPaged) dst = static_cast<T*>(a.o_split) + rowi * a.head_dim;
-        else dst32 = static_cast<float*>(a.o_split) + rowi * a.head_dim;
-        if (row_valid) {
+        // Four columns of all rows together, so that a warp's store is one run of memory.
+        else dst32 = static_cast<float*>(a.o_split) +
+                     (static_cast<int64_t>(e.slot) * (a.head_dim / 4) * kUnitRows + q_tile * kAttnTileM + row) * 4;
+        if (row_valid && (kForm == kFormPaged || !dual || t == 0)) {
           a.m_split[rowi] = (l > 0.f) ? m_used * 0.69314718055994530942f : -INFINITY;
           a.l_split[rowi] = l;
         }
@@ -978,34 +1338,58 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
       for (int c4 = 0; c4 < (kWide ? 8 : kNarrow ? 2 : 4); ++c4) {
         if (c4 * 32 >= a.head_dim) break;  // warp-uniform: only the row's real columns
+        if (kStreamed && dual && (c4 >= (kNarrow ? 1 : 2)) != (t == 1)) continue;  // the other group's half
         uint32_t o[32];
         if (n_tiles > 0) {
-          tmem_ld32(o_addr + 32 * c4, o);
+          // In a single-tile unit of one KV tile group 1 has no O: both read group 0's.
+          const bool own_o = !kStreamed || own > 0;
+          tmem_ld32((own_o ? o_addr : o_addr - 128) + 32 * c4, o);
           tmem_wait_ld(o);
+          if (kStreamed && join) {
+            uint32_t o1[32];
+            tmem_ld32((t == 0 ? o_addr + 128 : o_addr - 128) + 32 * c4, o1);
+            tmem_wait_ld(o1);
+#pragma unroll
+            for (int cc = 0; cc < 32; ++cc) {
+              // A group that saw no key has weight 0, whatever its O holds.
+              const float x1 = w_other != 0.f ? __uint_as_float(o1[cc]) * w_other : 0.f;
+              o[cc] = __float_as_uint((w_self != 0.f ? __uint_as_float(o[cc]) * w_self : 0.f) + x1);
+            }
+          } else {
+            const float w = own_o ? w_self : w_other;
+#pragma unroll
+            for (int cc = 0; cc < 32; ++cc) o[cc] = __float_as_uint(__uint_as_float(o[cc]) * w);
+          }
         } else {
 #pragma unroll
           for (int cc = 0; cc < 32; ++cc) o[cc] = 0u;
         }
         if (kForm != kFormPaged && dst32) {
           if (row_valid) {
-            float4* f4 = reinterpret_cast<float4*>(dst32 + c4 * 32);
 #pragma unroll
             for (int v = 0; v < 8; ++v)
-              f4[v] = make_float4(__uint_as_float(o[4 * v]) * inv, __uint_as_float(o[4 * v + 1]) * inv,
-                                  __uint_as_float(o[4 * v + 2]) * inv, __uint_as_float(o[4 * v + 3]) * inv);
+              reinterpret_cast<float4*>(dst32)[static_cast<int64_t>(c4 * 8 + v) * kUnitRows] =
+                  make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]), __uint_as_float(o[4 * v + 2]),
+                              __uint_as_float(o[4 * v + 3]));
           }
         } else if (row_valid) {
-          uint4* d4 = reinterpret_cast<uint4*>(dst + c4 * 32);
+          uint32_t w[16];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint4 w;
-            w.x = Pack2<T>::pack(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv);
-            w.y = Pack2<T>::pack(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
-            w.z = Pack2<T>::pack(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
-            w.w = Pack2<T>::pack(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
-            d4[v] = w;
+          for (int v = 0; v < 16; ++v) w[v] = Pack2<T>::pack(__uint_as_float(o[2 * v]), __uint_as_float(o[2 * v + 1]));
+          if (kStreamed && a.wide_out) {  // whole 32-byte sectors
+            st_global_v8(dst + c4 * 32, w);
+            st_global_v8(dst + c4 * 32 + 16, w + 8);
+          } else {
+            uint4* d4 = reinterpret_cast<uint4*>(dst + c4 * 32);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) d4[v] = make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
           }
         }
+      }
+      if (kStreamed && dual) {  // both O are read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(BAR_ML_DONE));
       }
     }
   }

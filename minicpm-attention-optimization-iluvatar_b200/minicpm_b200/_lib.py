@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 from pathlib import Path
@@ -295,7 +296,8 @@ def check(status: int, what: str) -> None:
 
 
 def current_stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 _NO_SWITCH = contextlib.nullcontext()
@@ -309,16 +311,10 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
-def row_strides(t: torch.Tensor, strides: tuple) -> tuple[int, int]:
-    """(row, head) strides of ``[rows, heads, D]``; a dimension of one element counts as packed."""
-    sh = strides[1] if t.shape[1] != 1 else t.shape[2]
-    return (strides[0] if t.shape[0] != 1 else t.shape[1] * sh), sh
-
-
-def page_strides(t: torch.Tensor, strides: tuple) -> tuple[int, int, int]:
-    """(block, token, head) strides of ``[blocks, block, heads, D]``; a dimension of one element counts as packed."""
-    sh = strides[2] if t.shape[2] != 1 else t.shape[3]
-    return (strides[0] if t.shape[0] != 1 else t.shape[1] * strides[1]), strides[1], sh
+@functools.lru_cache(maxsize=256)
+def varlen_workspace_bytes(device_index: int, *sizes: int) -> int:
+    """``b200_varlen_attn_workspace_bytes`` of these sizes (it asks the current device for its SM count)."""
+    return int(load().b200_varlen_attn_workspace_bytes(*sizes))
 
 
 def device_error(device: torch.device | None = None) -> int:

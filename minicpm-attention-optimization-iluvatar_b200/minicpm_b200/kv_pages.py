@@ -32,48 +32,50 @@ class CacheLayers:
     """
 
     def __init__(self, kv_caches: Sequence[torch.Tensor]):
-        views: list[torch.Tensor] = []
-        for cache in kv_caches:
-            if cache.ndim == 5 and cache.shape[1] == 2:
-                views += [cache[:, 0], cache[:, 1]]
-            elif cache.ndim == 4:
-                views.append(cache)
-            else:
-                raise ValueError("a cache is [num_blocks, 2, block_size, kv_heads, D] or [num_blocks, block_size, kv_heads, D]")
-        if not 1 <= len(views) <= 256:
+        caches = list(kv_caches)
+        if not caches:
             raise ValueError("1 to 256 K/V tensors (128 layers) in one set of caches")
-        first = views[0]
-        for t in views:
-            if t.shape != first.shape or t.stride() != first.stride() or t.dtype != first.dtype or t.device != first.device:
+        first = caches[0]
+        shape, strides, dtype, device = first.shape, first.stride(), first.dtype, first.device
+        paired = len(shape) == 5 and shape[1] == 2
+        if not paired and len(shape) != 4:
+            raise ValueError("a cache is [num_blocks, 2, block_size, kv_heads, D] or [num_blocks, block_size, kv_heads, D]")
+        e = first.element_size()
+        base: list[int] = []
+        for t in caches:
+            if t.shape != shape or t.stride() != strides or t.dtype != dtype or t.device != device:
                 raise ValueError("all caches must share shape, strides, dtype and device")
-        if first.numel() == 0 or (first.stride(3) != 1 and first.shape[3] != 1):
+            base.append(t.data_ptr())
+            if paired:
+                base.append(base[-1] + strides[1] * e)
+        if len(base) > 256:
+            raise ValueError("1 to 256 K/V tensors (128 layers) in one set of caches")
+        n, block, heads, row = (shape[0], *shape[2:]) if paired else shape
+        sb, st, sh, sd = (strides[0], *strides[2:]) if paired else strides
+        if n * block * heads * row == 0 or (sd != 1 and row != 1):
             raise ValueError("the caches must not be empty and their rows must be contiguous")
-        if len({t.data_ptr() for t in views}) != len(views):
+        if len(set(base)) != len(base):
             raise ValueError("a cache is named twice")
-        n, block, heads, row = first.shape
-        sb, st, sh, _ = first.stride()
-        row_run = row
         page = block * heads * row
-        nhd = (heads == 1 or sh == row_run) and (block == 1 or st == heads * row_run)
-        hnd = (block == 1 or st == row_run) and (heads == 1 or sh == block * row_run)
+        nhd = (heads == 1 or sh == row) and (block == 1 or st == heads * row)
+        hnd = (block == 1 or st == row) and (heads == 1 or sh == block * row)
         if not (nhd or hnd) or (n > 1 and sb < page):
             raise ValueError("a page must be one dense run of [block_size, kv_heads, D] or [kv_heads, block_size, D]")
-        e = first.element_size()
+        # A dimension of one element may carry any stride: the library gets the dense one.
         if n == 1:
             sb = page
-        # A dimension of one element may carry any stride: the library gets the dense one.
         if block == 1:
-            st = heads * row_run if nhd else row_run
+            st = heads * row if nhd else row
         if heads == 1:
-            sh = row_run
-        if (page * e) % 4 or (sb * e) % 4 or (row * e) % 4 or any(t.data_ptr() % 4 for t in views):
+            sh = row
+        if (sb * e) % 4 or (row * e) % 4 or any(b % 4 for b in base):
             raise ValueError("cache rows must be 4-byte aligned")
-        self.tensors = list(kv_caches)
-        self.device = first.device
+        self.tensors = caches
+        self.device = device
         self.num_blocks, self.block_size = n, block
-        self._base = (ctypes.c_void_p * len(views))(*(t.data_ptr() for t in views))
-        self.params = _lib.PageCaches(ctypes.cast(self._base, ctypes.c_void_p), len(views), n, block, heads, row * e,
-                                      sb * e, st * e, sh * e)
+        self._base = (ctypes.c_void_p * len(base))(*base)
+        self.params = _lib.PageCaches(ctypes.cast(self._base, ctypes.c_void_p), len(base), n, block, heads, row * e, sb * e,
+                                      st * e, sh * e)
         self._ref = ctypes.byref(self.params)
 
 
@@ -91,25 +93,30 @@ def cache_layers(kv_caches: Caches) -> CacheLayers:
     return kv_caches if isinstance(kv_caches, CacheLayers) else CacheLayers(kv_caches)
 
 
+_INDEX_TYPES = (torch.int32, torch.int64)
+
+
 def _indices(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if t.ndim != 1 or t.dtype not in (torch.int32, torch.int64):
+    if t.ndim != 1 or t.dtype not in _INDEX_TYPES:
         raise ValueError(f"{name} must be a one-dimensional int32 or int64 tensor")
     if t.device != device:
         raise ValueError(f"{name} must be on the same device as the table or caches")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _table(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: Optional[torch.Tensor], num_blocks: int,
            block_size: int) -> "_lib.SeqTable":
-    dev = block_table.device
-    if block_table.ndim != 2 or block_table.dtype not in (torch.int32, torch.int64) or block_table.shape[1] == 0:
+    if block_table.ndim != 2 or block_table.dtype not in _INDEX_TYPES or block_table.shape[1] == 0:
         raise ValueError("block_table must contain integer physical block ids, [max_seqs, max_pages]")
-    if block_table.stride(1) != 1 or (block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]):
+    rows, cols = block_table.shape
+    stride, step = block_table.stride()
+    if step != 1 or (rows > 1 and stride < cols):
         raise ValueError("block_table is written in place: its rows must be contiguous and apart")
-    if seq_lens.ndim != 1 or seq_lens.shape[0] != block_table.shape[0] or seq_lens.dtype not in (torch.int32, torch.int64):
+    if seq_lens.ndim != 1 or seq_lens.shape[0] != rows or seq_lens.dtype not in _INDEX_TYPES:
         raise ValueError("seq_lens must hold one int32 or int64 length per row of the block table")
     if not seq_lens.is_contiguous():
         raise ValueError("seq_lens is written in place: it must be contiguous")
+    dev = block_table.device
     if seq_lens.device != dev:
         raise ValueError("block_table and seq_lens must be on the same device")
     refs = None
@@ -119,9 +126,8 @@ def _table(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: Option
         if not ref_counts.is_contiguous() or ref_counts.device != dev:
             raise ValueError("ref_counts is written in place: contiguous, on the table's device")
         refs = ref_counts.data_ptr()
-    return _lib.SeqTable(block_table.data_ptr(), seq_lens.data_ptr(), refs,
-                         max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], block_table.shape[0],
-                         num_blocks, block_size, _lib.dtype_code(block_table.dtype), _lib.dtype_code(seq_lens.dtype))
+    return _lib.SeqTable(block_table.data_ptr(), seq_lens.data_ptr(), refs, stride if rows > 1 else max(stride, cols), cols,
+                         rows, num_blocks, block_size, _lib.dtype_code(block_table.dtype), _lib.dtype_code(seq_lens.dtype))
 
 
 def _same_device(layers: CacheLayers, dev: torch.device) -> None:

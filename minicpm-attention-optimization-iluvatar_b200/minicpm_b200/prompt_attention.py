@@ -20,6 +20,9 @@ import torch
 
 from . import _lib
 
+_INDEX_TYPES = (torch.int32, torch.int64)
+_ELEMENT_TYPES = (torch.bfloat16, torch.float16)
+
 
 def prompt_attention(
     q: torch.Tensor,
@@ -52,50 +55,61 @@ def prompt_attention(
     """
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
         raise ValueError("expected q=[T,H,D] and k/v=[Tk,kv_heads,D]")
-    if out.shape != q.shape or k.shape != v.shape:
+    q_shape, k_shape = q.shape, k.shape
+    if out.shape != q_shape or k_shape != v.shape:
         raise ValueError("out must match q and k/v must have identical shapes")
     same_k = cu_seqlens_k is None
     if same_k:
         cu_seqlens_k = cu_seqlens_q
     dev = q.device
-    if k.device != dev or v.device != dev or out.device != dev or cu_seqlens_q.device != dev or cu_seqlens_k.device != dev:
+    if not (dev == k.device == v.device == out.device == cu_seqlens_q.device == cu_seqlens_k.device):
         raise ValueError("all tensors must be on the same device")
     if cu_seqlens_q.ndim != 1 or cu_seqlens_q.shape != cu_seqlens_k.shape or cu_seqlens_q.shape[0] < 1:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must contain one entry per sequence plus one")
-    if cu_seqlens_q.dtype != cu_seqlens_k.dtype or cu_seqlens_q.dtype not in (torch.int32, torch.int64):
+    len_dtype = cu_seqlens_q.dtype
+    if cu_seqlens_k.dtype != len_dtype or len_dtype not in _INDEX_TYPES:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must be int32 or int64 of one dtype")
-    total_q, hq, head_dim = q.shape
-    total_k, hkv, dk = k.shape
+    total_q, hq, head_dim = q_shape
+    total_k, hkv, dk = k_shape
     if dk != head_dim or head_dim not in (64, 128, 256) or hkv == 0 or hq == 0 or hq % hkv:
         raise ValueError("unsupported head shape for prompt attention")
     if same_k and total_k < total_q:
         raise ValueError("k and v hold fewer rows than q: pass cu_seqlens_k")
     if max_seqlen_k is None:
         max_seqlen_k = max_seqlen_q if same_k else total_k
-    if not softmax_scale > 0.0 or softmax_scale > 3.0e38:
+    if not 0.0 < softmax_scale <= 3.0e38:
         raise ValueError("softmax_scale must be positive and finite")
-    if dev.type != "cuda":
+    if not q.is_cuda:
         raise RuntimeError("prompt_attention runs on CUDA tensors only (no CPU path)")
     dtype = q.dtype
-    if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
+    if dtype not in _ELEMENT_TYPES or not (dtype == k.dtype == v.dtype == out.dtype):
         raise RuntimeError("the sm_100a kernel takes bf16 or f16 q/k/v/out of one dtype")
-    qs, ks, vs, outs = q.stride(), k.stride(), v.stride(), out.stride()
-    if qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or outs[2] != 1:
+    (qt, qh, qd), (kt, kh, kd), (vt, vh, vd), (ot, oh, od) = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (qd == kd == vd == od == 1):
         raise RuntimeError("the head dimension of q, k, v and out must be contiguous")
     num_seqs = cu_seqlens_q.shape[0] - 1
     if total_q == 0 or num_seqs == 0:
         return out
-    cu_seqlens_q = cu_seqlens_q.contiguous()
-    cu_seqlens_k = cu_seqlens_k.contiguous()
+    # A dimension of one element may carry any stride: it counts as packed.
+    if hq == 1:
+        qh = oh = head_dim
+    if hkv == 1:
+        kh = vh = head_dim
+    if total_q == 1:
+        qt, ot = hq * qh, hq * oh
+    if total_k == 1:
+        kt, vt = hkv * kh, hkv * vh
+    if not (cu_seqlens_q.is_contiguous() and cu_seqlens_k.is_contiguous()):
+        cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
+    max_seqlen_k = int(max_seqlen_k)
     lib = _lib.load()
     with _lib.on_device(dev):
-        nbytes = lib.b200_varlen_attn_workspace_bytes(total_q, num_seqs, hq, hkv, head_dim, int(max_seqlen_k))
+        nbytes = _lib.varlen_workspace_bytes(dev.index, total_q, num_seqs, hq, hkv, head_dim, max_seqlen_k)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         p = _lib.PromptAttnParams(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-            *_lib.row_strides(q, qs), *_lib.row_strides(k, ks), *_lib.row_strides(v, vs), *_lib.row_strides(out, outs),
-            _lib.dtype_code(cu_seqlens_q.dtype), _lib.dtype_code(dtype), num_seqs, total_q, total_k, hq, hkv, head_dim,
-            int(max_seqlen_k), int(bool(causal)), float(softmax_scale), ws.data_ptr(), nbytes,
+            qt, qh, kt, kh, vt, vh, ot, oh, _lib.dtype_code(len_dtype), _lib.dtype_code(dtype), num_seqs, total_q, total_k,
+            hq, hkv, head_dim, max_seqlen_k, bool(causal), softmax_scale, ws.data_ptr(), nbytes,
         )
         _lib.check(lib.b200_prompt_attn_fwd(ctypes.byref(p), _lib.current_stream(dev)), "prompt_attention")
     return out
