@@ -15,6 +15,10 @@ same signature, same feature guards, same routing, same exceptions.
   scale caches) takes the optimized path too: its referenced pages are
   dequantised (``b200_kv_dequant_pages``) and attended by the same kernel.
   The reference routes every quantised cache to vLLM.
+* ``tree_mask`` (new) marks the query rows as drafted token trees (speculative
+  decoding): the call runs :func:`~minicpm_b200.paged_tree_attention`, single
+  tokens included, and raises ``RuntimeError`` when the flags are off or an
+  unsupported feature is requested -- no baseline takes a tree.
 * A head shape or element type the sm_100a kernel does not run (fp32,
   head_dim other than 64 / 128 / 256, more than 128 query heads per KV head;
   ``kernel_supports``)
@@ -129,6 +133,8 @@ def iluvatar_attention(
     cos_cache: Optional[torch.Tensor] = None,
     sin_cache: Optional[torch.Tensor] = None,
     rotary_dim: Optional[int] = None,
+    # Draft trees [total_q, >= max_seqlen_q] (bool or uint8)
+    tree_mask: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Route one attention call; returns ``out`` (written in place)."""
     original_k, original_v = k, v
@@ -139,7 +145,7 @@ def iluvatar_attention(
         not use_optimized()
         or not split_kv_enabled()
         or max_seqlen_q < 1
-        or (max_seqlen_q == 1 and not decode_enabled())
+        or (max_seqlen_q == 1 and not decode_enabled() and tree_mask is None)
         or softcap != 0.0
         or not _quantised_cache_supported(kv_quant_mode, k_descale, v_descale, k_scale_cache, v_scale_cache)
         or alibi_slopes is not None
@@ -150,6 +156,11 @@ def iluvatar_attention(
         or not kernel_supports(q, k, kv_quant_mode)
     )
 
+    if use_baseline and tree_mask is not None:
+        raise RuntimeError(
+            "draft-tree attention runs on the optimized path only: set ILUVATAR_USE_OPTIMIZED=1 and "
+            "ILUVATAR_SPLIT_KV=1, and request no feature or head shape that path lacks"
+        )
     if use_baseline:
         unified_attention = _vllm_unified_attention()
         if unified_attention is None:
@@ -208,6 +219,7 @@ def iluvatar_attention(
         v_descale=v_descale,
         k_scale_cache=k_scale_cache,
         v_scale_cache=v_scale_cache,
+        tree_mask=tree_mask,
     )
 
 

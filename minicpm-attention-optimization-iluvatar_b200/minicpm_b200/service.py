@@ -19,6 +19,9 @@ reference's integration patch adds it (``integration/vllm-plugin-FL-split-kv.pat
   encoder attention, per-token-head and fp8 caches, the call above),
   ``do_kv_cache_update`` (the sm_100a cache writers of :mod:`.kv_cache`) and
   ``do_rope_and_kv_cache_update`` (the fused RoPE + cache write).
+  Encoder batches run :func:`~minicpm_b200.prompt_attention` when both flags are
+  set and the call has no sliding window, bias or unsupported shape, else vLLM's
+  ``context_attention_fwd`` as in the reference.
 * :class:`IluvatarAttentionMetadata`, :class:`IluvatarAttentionMetadataBuilder`
   and :class:`IluvatarAttentionBackend` (patch :150-466) -- the metadata, its
   builder and the backend's static contract (cache shape and stride order,
@@ -37,6 +40,10 @@ Differences from the reference, on purpose:
   route treats any descale as unsupported, so the optimized path was never
   taken in the service (``docs/stage-summary-2026-10-09.md``, section 6).  Here
   the descales are passed only when the cache is quantised.
+* ``tree_mask`` in the metadata (the builder takes it from the scheduler's common
+  metadata when that has one) marks the step's query tokens as drafted trees: the
+  step runs :func:`~minicpm_b200.paged_tree_attention` and raises ``RuntimeError``
+  where the sm_100a path cannot take it.
 * ``ILUVATAR_NUM_SPLITS`` unset means an automatically chosen split count
   (the reference used 4).
 * ``fused_rope_kvcache_supported`` is true for every cache except the
@@ -65,6 +72,7 @@ from .kv_cache import (
     reshape_and_cache_flash_per_token_head_quant,
     rope_and_cache,
 )
+from .prompt_attention import prompt_attention
 from .split_kv_paged import kernel_supports
 from .unified_attention_optimized import unified_attention_optimized
 
@@ -122,6 +130,7 @@ def _vllm_unified_attention():
 def _run_unified_attention(**kwargs: Any) -> torch.Tensor:
     """Use the sm_100a path for supported prefill / mixed (and, if enabled, decode) calls."""
     enabled = _flag("ILUVATAR_USE_OPTIMIZED") and _flag("ILUVATAR_SPLIT_KV")
+    tree_mask = kwargs.pop("tree_mask", None)
     max_query_len = kwargs["max_seqlen_q"]
     mode = KVQuantMode(int(kwargs.get("kv_quant_mode", KVQuantMode.NONE)))
     # Descales belong to the fp8 per-tensor cache (its dequantisation scales);
@@ -142,7 +151,9 @@ def _run_unified_attention(**kwargs: Any) -> torch.Tensor:
         or kwargs.get("causal") is not True
         or not kernel_supports(kwargs["q"], kwargs["k"], int(mode))
     )
-    decode_only = max_query_len <= 1
+    decode_only = max_query_len <= 1 and tree_mask is None
+    if tree_mask is not None and (not enabled or unsupported or max_query_len < 1):
+        raise RuntimeError("draft-tree attention runs on the sm_100a path only, which is off or lacks a requested feature")
     if not enabled or unsupported or max_query_len < 1 or (decode_only and not _flag("ILUVATAR_SPLIT_KV_DECODE")):
         return _vllm_unified_attention()(**kwargs)
     num_splits = int(os.environ.get("ILUVATAR_NUM_SPLITS", "0") or 0)
@@ -168,6 +179,7 @@ def _run_unified_attention(**kwargs: Any) -> torch.Tensor:
         v_descale=kwargs.get("v_descale"),
         k_scale_cache=kwargs.get("k_scale_cache"),
         v_scale_cache=kwargs.get("v_scale_cache"),
+        **({} if tree_mask is None else {"tree_mask": tree_mask}),
     )
 
 
@@ -201,6 +213,7 @@ class IluvatarAttentionMetadata:
     prefix_scheduler_metadata: torch.Tensor | None = None
     mm_prefix_range: dict[int, list[tuple[int, int]]] | None = None
     mm_prefix_range_tensor: torch.Tensor | None = None
+    tree_mask: torch.Tensor | None = None  # drafted token trees [num_actual_tokens, >= max_query_len]
 
 
 def _next_power_of_2(n: int) -> int:
@@ -266,6 +279,7 @@ class IluvatarAttentionMetadataBuilder:
         ranges = getattr(common, "mm_req_doc_ranges", None)
         if ranges is not None:
             meta.mm_prefix_range = ranges
+        meta.tree_mask = getattr(common, "tree_mask", None)
         return meta
 
     def build_for_cudagraph_capture(self, common: Any) -> IluvatarAttentionMetadata:
@@ -494,13 +508,20 @@ class IluvatarAttentionImpl:
             v_scale_cache=v_scale_cache,
             chunk_lookback=self.chunk_lookback,
             use_td=self.use_td,
+            **({} if attn_metadata.tree_mask is None else {"tree_mask": attn_metadata.tree_mask[:n]}),
         )
         return output
 
     def _forward_encoder_attention(self, query, key, value, output, attn_metadata, layer) -> torch.Tensor:
-        """Bidirectional attention without a cache: vLLM's ``context_attention_fwd``, as in the reference."""
+        """Bidirectional attention without a cache: ``prompt_attention`` (both flags set, no window or
+        bias, a shape the kernel runs), else vLLM's ``context_attention_fwd`` as in the reference."""
         if is_quantized_kv_cache(self.kv_cache_dtype):
             raise NotImplementedError("quantized KV cache is not supported for encoder attention")
+        if (_flag("ILUVATAR_USE_OPTIMIZED") and _flag("ILUVATAR_SPLIT_KV") and self.sliding_window == (-1, -1)
+                and self.alibi_slopes is None and self.sinks is None and not self.logits_soft_cap
+                and kernel_supports(query, key.unsqueeze(0)) and value.dtype == query.dtype == output.dtype):
+            return prompt_attention(query, key, value, output, attn_metadata.query_start_loc, attn_metadata.max_query_len,
+                                    self.scale, causal=False)
         try:
             from vllm.v1.attention.ops.triton_prefill_attention import context_attention_fwd
         except Exception as exc:

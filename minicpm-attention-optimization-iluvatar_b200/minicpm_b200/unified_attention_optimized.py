@@ -10,7 +10,10 @@ is chosen automatically (``0``) instead of the reference's fixed 4; and a
 quantised cache (``kv_quant_mode`` 1: fp8 per-tensor with ``k_descale`` /
 ``v_descale``; 2 / 3: int8 / fp8 per-token-head with ``k_scale_cache`` /
 ``v_scale_cache``), which the reference leaves to vLLM, is dequantised page by
-page (``b200_kv_dequant_pages``) and attended by the same kernel.
+page (``b200_kv_dequant_pages``) and attended by the same kernel.  With
+``tree_mask`` (new) the query rows are drafted token trees and the call goes to
+:func:`~minicpm_b200.paged_tree_attention`, quantised caches included; the split
+count is then the library's own.
 """
 
 from __future__ import annotations
@@ -22,6 +25,7 @@ import torch
 
 from .kv_cache import dequantize_kv_pages
 from .split_kv_paged import paged_split_kv_attention
+from .tree_attention import paged_tree_attention
 
 
 def resolve_num_splits(override: Optional[int]) -> int:
@@ -55,6 +59,7 @@ def unified_attention_optimized(
     v_descale: Optional[torch.Tensor] = None,
     k_scale_cache: Optional[torch.Tensor] = None,
     v_scale_cache: Optional[torch.Tensor] = None,
+    tree_mask: Optional[torch.Tensor] = None,
     **kwargs,
 ) -> torch.Tensor:
     if causal is not True:
@@ -66,6 +71,9 @@ def unified_attention_optimized(
             k, v, block_table, seqused_k, max_seqlen_k, kv_quant_mode, q.dtype, q.shape[2],
             k_descale=k_descale, v_descale=v_descale, k_scale_cache=k_scale_cache, v_scale_cache=v_scale_cache)
         k, v = dense[:, 0], dense[:, 1]
+    if tree_mask is not None:
+        return paged_tree_attention(q, k, v, out, tree_mask, block_table, seqused_k, cu_seqlens_q, max_seqlen_q,
+                                    max_seqlen_k, softmax_scale)
     return paged_split_kv_attention(
         q=q,
         k=k,

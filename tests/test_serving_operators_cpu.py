@@ -231,3 +231,88 @@ def test_the_oracles_agree_with_the_paged_one():
     rows = cache[table[0]].transpose(0, 1).reshape(2, -1, 2, 64)[:, :L]
     plain, _, _ = prompt_attention_reference(q, rows[0], rows[1], [0, 7], [0, L], 0.3, True)
     assert (plain - tree).abs().max() < 1e-12
+
+
+# ------------------------------------------------------------------ routes
+def _flags(monkeypatch, on=True):
+    for name in ("ILUVATAR_USE_OPTIMIZED", "ILUVATAR_SPLIT_KV"):
+        if on:
+            monkeypatch.setenv(name, "1")
+        else:
+            monkeypatch.delenv(name, raising=False)
+    monkeypatch.delenv("ILUVATAR_SPLIT_KV_DECODE", raising=False)
+
+
+@pytest.mark.parametrize("max_q", [1, 9])
+def test_dispatcher_sends_trees_to_the_optimized_path(monkeypatch, max_q):
+    from minicpm_b200 import attention
+
+    seen = {}
+    monkeypatch.setattr(attention, "unified_attention_optimized", lambda **kw: seen.update(kw))
+    monkeypatch.setattr(attention, "_vllm_unified_attention", lambda: pytest.fail("a tree has no baseline"))
+    q, k = torch.zeros(9, 16, 128, dtype=BF), torch.zeros(4, 16, 2, 128, dtype=BF)
+    mask = torch.ones(9, 9, dtype=torch.bool)
+    args = (q, k, k, q, None, max_q, None, 64, 0.1)
+    _flags(monkeypatch, False)
+    with pytest.raises(RuntimeError, match="optimized path only"):
+        minicpm_b200.iluvatar_attention(*args, tree_mask=mask)
+    _flags(monkeypatch)
+    minicpm_b200.iluvatar_attention(*args, tree_mask=mask)
+    assert seen["tree_mask"] is mask and seen["max_seqlen_q"] == max_q
+    with pytest.raises(RuntimeError, match="optimized path only"):
+        minicpm_b200.iluvatar_attention(*args, tree_mask=mask, softcap=30.0)
+
+
+def test_service_routes_trees_and_encoders(monkeypatch):
+    from types import SimpleNamespace
+
+    from minicpm_b200 import service
+
+    calls = []
+    monkeypatch.setattr(service, "unified_attention_optimized", lambda **kw: calls.append(("tree", kw)))
+    monkeypatch.setattr(service, "_vllm_unified_attention", lambda: (lambda **kw: calls.append(("vllm", kw))))
+    monkeypatch.setattr(service, "prompt_attention", lambda *a, **kw: calls.append(("prompt", a, kw)))
+    q, k = torch.zeros(9, 16, 128, dtype=BF), torch.zeros(4, 16, 2, 128, dtype=BF)
+    mask = torch.ones(9, 9, dtype=torch.bool)
+    base = dict(q=q, k=k, v=k, out=q, cu_seqlens_q=None, max_seqlen_q=1, seqused_k=None, max_seqlen_k=64, softmax_scale=0.1,
+                causal=True, block_table=None)
+    _flags(monkeypatch, False)
+    with pytest.raises(RuntimeError, match="sm_100a path only"):
+        service._run_unified_attention(**base, tree_mask=mask)
+    service._run_unified_attention(**base, tree_mask=None)
+    assert calls[-1][0] == "vllm" and "tree_mask" not in calls[-1][1]
+    _flags(monkeypatch)
+    service._run_unified_attention(**base, tree_mask=mask)
+    assert calls[-1][0] == "tree" and calls[-1][1]["tree_mask"] is mask
+    with pytest.raises(RuntimeError, match="sm_100a path only"):
+        service._run_unified_attention(**{**base, "causal": False}, tree_mask=mask)
+
+    # The metadata carries the mask of the step; a scheduler without one leaves it out.
+    common = SimpleNamespace(num_reqs=1, num_actual_tokens=9, max_query_len=9, max_seq_len=64,
+                             query_start_loc=torch.tensor([0, 9]), seq_lens=torch.tensor([64]),
+                             block_table_tensor=torch.zeros(1, 4), slot_mapping=None, causal=True)
+    builder = service.IluvatarAttentionMetadataBuilder(16, 2, 128, torch.device("cpu"))
+    assert builder.build(0, common).tree_mask is None
+    common.tree_mask = torch.ones(12, 9, dtype=torch.bool)  # padded like the step's tensors
+    meta = builder.build(0, common)
+    impl = service.IluvatarAttentionImpl(16, 128, 0.1, 2, None, None, "auto")
+    impl.forward(SimpleNamespace(), q, q, q, torch.zeros(4, 2, 16, 2, 128, dtype=BF), meta, torch.empty_like(q))
+    assert calls[-1][0] == "tree" and calls[-1][1]["tree_mask"].shape == (9, 9)
+
+    # Encoder batches: the sm_100a kernel with both flags and a plain call, else vLLM's.
+    meta.tree_mask = None
+    enc = service.IluvatarAttentionImpl(16, 128, 0.1, 2, None, None, "auto", attn_type=service.AttentionType.ENCODER_ONLY)
+    kv = torch.zeros(9, 2, 128, dtype=BF)
+    enc.forward(SimpleNamespace(), q, kv, kv, torch.zeros(0), meta, torch.empty_like(q))
+    assert calls[-1][0] == "prompt" and calls[-1][2] == {"causal": False}
+    count = len(calls)
+    for over in (dict(sliding_window=128), dict(alibi_slopes=[0.1] * 16), dict(logits_soft_cap=30.0)):
+        args = dict(alibi_slopes=None, sliding_window=None, logits_soft_cap=None)
+        args.update(over)
+        other = service.IluvatarAttentionImpl(16, 128, 0.1, 2, args["alibi_slopes"], args["sliding_window"], "auto",
+                                              args["logits_soft_cap"], attn_type=service.AttentionType.ENCODER_ONLY)
+        try:
+            other.forward(SimpleNamespace(), q, kv, kv, torch.zeros(0), meta, torch.empty_like(q))
+        except Exception:
+            pass  # vLLM's kernel does not run here
+        assert len(calls) == count
