@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kCombineThreads) stream_combine_kernel(const S
 namespace b200_host {
 
 struct FormLayout {
-  bool streamed;
+  bool streamed, shares;  // shares: a unit may be shared by CTAs
   int ctas, ppt, ppu;
   int64_t qunits_ub, capacity;
   // streamed: CTAs' shared units and partials
@@ -161,8 +161,11 @@ inline FormLayout form_layout(bool tree, int64_t total_q, int num_seqs, int hq, 
       std::max<int64_t>((total_q + w.ppu - 1) / w.ppu, std::min<int64_t>(num_seqs, total_q)) * hkv;
   w.streamed = tree || units_lb < sms || (units_lb < (int64_t)kStreamRounds * sms && tiles >= kStreamLongTiles);
   w.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(w.streamed ? ticks / b200::kStreamMinTicks : w.capacity, sms));
+  // No unit as long as two pieces (by the caller's bound): none is shared, and there
+  // is nothing to join.
+  w.shares = w.streamed && w.ctas > 1 && tiles >= 2 * b200::kStreamMinTiles;
   if (w.streamed) {
-    const size_t rows = (size_t)2 * w.ctas * b200::kUnitRows;
+    const size_t rows = w.shares ? (size_t)2 * w.ctas * b200::kUnitRows : 0;
     w.o_off = align_up(sizeof(int4) * (size_t)w.ctas, 256);
     w.m_off = w.o_off + rows * head_dim * sizeof(float);
     w.l_off = w.m_off + rows * sizeof(float);
@@ -307,6 +310,7 @@ int run_form(FormLaunch& f, const FormLayout& w, int64_t max_tiles, int sms, cud
   a.num_kv_heads = f.num_kv_heads;
   a.num_splits = 1;
   a.wide_out = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.out_st * 2) | (uintptr_t)(a.out_sh * 2)) & 31) == 0;
+  a.min_piece = w.shares ? b200::kStreamMinTiles : 0x3fffffff;
   if constexpr (b200::form_streamed(kForm)) {
     a.stream_meta = reinterpret_cast<int4*>(ws);
     a.o_split = ws + w.o_off;
@@ -325,7 +329,7 @@ int run_form(FormLaunch& f, const FormLayout& w, int64_t max_tiles, int sms, cud
     r = bf16 ? launch_attn_dim<__nv_bfloat16, kMaps, kForm>(f, grid, s) : launch_attn_dim<__half, kMaps, kForm>(f, grid, s);
   else
     r = bf16 ? launch_attn_dim<__nv_bfloat16, false, kForm>(f, grid, s) : launch_attn_dim<__half, false, kForm>(f, grid, s);
-  if (r != B200_OK || !b200::form_streamed(kForm) || w.ctas == 1) return r;  // one CTA shares no unit
+  if (r != B200_OK || !w.shares) return r;
 
   if constexpr (b200::form_streamed(kForm)) {
     b200::StreamCombineArgs c{};

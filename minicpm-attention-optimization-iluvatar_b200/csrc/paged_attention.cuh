@@ -166,7 +166,7 @@ __device__ __forceinline__ void unpack_unit(const int4 u, int& kvh, int& split, 
 constexpr int kUnitRows = 256;  // partial rows per split unit: 2 query tiles x 128 rows
 constexpr uint32_t kSmRing = BAR_COUNT * 8 + 16;  // after the barriers, the TMEM slot and the abort flag
 static_assert(kSmRing + kUnitRing * sizeof(UnitEntry) <= 512, "barrier area");
-static_assert(kSmRing % 8 == 0 && kUnitRing * sizeof(UnitEntry) >= kAttnThreads / 32 * 8 + 6 * 4, "scratch of stream_share");
+static_assert(kSmRing % 8 == 0 && kUnitRing * sizeof(UnitEntry) >= (kAttnThreads / 32 + 6) * 4, "scratch of stream_share_block");
 
 struct AttnKernelArgs {
   const void* block_table;
@@ -200,6 +200,7 @@ struct AttnKernelArgs {
   int total_k;
   int full;                  // every row's keys end at L (bidirectional, or masked by the tree)
   int wide_out;              // rows of out are 32-byte aligned
+  int min_piece;             // streamed: KV tiles of a piece at least; no unit is shared where none has twice that
   int num_seqs, num_kv_heads;
   int4* stream_meta;         // [grid]: sequence, query unit, KV head, pieces of the unit that CTA i begins and does not end (0: none)
 };
@@ -316,6 +317,7 @@ __device__ __forceinline__ UnitGeom piece_geometry(int q_begin, int q_end, int s
 constexpr int kStreamOverhead = 2;
 constexpr int kStreamMinTicks = 3;  // a CTA's share at least
 constexpr int kStreamMinTiles = 2;  // KV tiles of a piece at least: fewer do not pay for its partial
+constexpr int kStreamWarpSeqs = 64;  // up to this many sequences the producer warp finds its share alone
 
 __device__ __forceinline__ int unit_weight(bool wide, int q_len, int qunit, int pos_per_unit) {
   return !wide && q_len - qunit * pos_per_unit > pos_per_unit / 2 ? 2 : 1;
@@ -375,11 +377,11 @@ __device__ __forceinline__ StreamUnit stream_unit(const AttnKernelArgs& a, const
 }
 
 // A share ends at a tile of the unit in which its raw tick falls, or at the unit's
-// start or end where fewer than kStreamMinTiles tiles would be left on that side.
-__device__ __forceinline__ int stream_snap(const StreamUnit& u, int x) {
-  const int tile = (x - u.first - kStreamOverhead) / u.weight;
-  if (x - u.first < kStreamOverhead || tile < kStreamMinTiles) return u.first;
-  if (u.tiles - tile < kStreamMinTiles) return u.first + u.ticks();
+// start or end where fewer than min_piece tiles would be left on that side.
+__device__ __forceinline__ int stream_snap(const StreamUnit& u, int x, int min_piece) {
+  const int tile = (x - u.first - kStreamOverhead) >> (u.weight - 1);
+  if (x - u.first < kStreamOverhead || tile < min_piece) return u.first;
+  if (u.tiles - tile < min_piece) return u.first + u.ticks();
   return u.first + kStreamOverhead + tile * u.weight;
 }
 
@@ -389,40 +391,93 @@ struct StreamShare {
   int x, end, seq, seq_first;
   int base, extra, ctas;
   __device__ __forceinline__ int raw(int i) const { return i * base + min(i, extra); }
+  __device__ __forceinline__ void divide(int total) {
+    ctas = max(1, min(static_cast<int>(gridDim.x), total / kStreamMinTicks));
+    base = total / ctas;
+    extra = total - base * ctas;
+  }
 };
 
-// Block-wide; scratch: 12 long longs and 6 ints of shared memory.  `mine`: the
-// bounds of sequence threadIdx.x (loaded early), if there is one.
+// Sums of ticks stop at 2^31 - 1: the host has bounded those of sequences that do
+// not overlap; of others the rest is dropped.
+__device__ __forceinline__ int add_ticks(int a, int b) {
+  return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), 0x7fffffffu));
+}
 template <int kForm, bool kWide>
-__device__ __forceinline__ StreamShare stream_share(const AttnKernelArgs& a, const SeqBounds& mine, int ppu,
-                                                    long long* scratch) {
-  const int per = (a.num_seqs + kAttnThreads - 1) / kAttnThreads;
-  const int s0 = min(static_cast<int>(threadIdx.x) * per, a.num_seqs), s1 = min(s0 + per, a.num_seqs);
-  long long ticks = 0;
-  for (int b = s0; b < s1; ++b) ticks += seq_ticks<kForm, kWide>(a, per == 1 ? mine : seq_bounds<kForm>(a, b), ppu);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long sum = ticks;
+__device__ __forceinline__ int seq_ticks_clipped(const AttnKernelArgs& a, const SeqBounds& sb, int ppu) {
+  return static_cast<int>(min(seq_ticks<kForm, kWide>(a, sb, ppu), 0x7fffffffll));
+}
+
+// The share, found by one warp: lane i holds the sequences 2 i and 2 i + 1 (mine,
+// loaded early).
+template <int kForm, bool kWide>
+__device__ __forceinline__ StreamShare stream_share_warp(const AttnKernelArgs& a, const SeqBounds (&mine)[2], int ppu) {
+  const int lane = threadIdx.x & 31;
+  const int t0 = 2 * lane < a.num_seqs ? seq_ticks_clipped<kForm, kWide>(a, mine[0], ppu) : 0;
+  const int t1 = 2 * lane + 1 < a.num_seqs ? seq_ticks_clipped<kForm, kWide>(a, mine[1], ppu) : 0;
+  int sum = add_ticks(t0, t1);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, sum, o);
-    if (lane >= o) sum += y;
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum = add_ticks(sum, y);
+  }
+  const int total = __shfl_sync(0xffffffffu, sum, 31);
+  int before = __shfl_up_sync(0xffffffffu, sum, 1);
+  if (lane == 0) before = 0;
+  StreamShare sh;
+  sh.divide(total);
+  sh.seq = a.num_seqs;
+  sh.seq_first = total;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int at = sh.raw(min(static_cast<int>(blockIdx.x) + k, sh.ctas));
+    const unsigned here = __ballot_sync(0xffffffffu, at >= before && at < sum);
+    int x = total;
+    if (here) {
+      const int src = __ffs(here) - 1;
+      const bool second = at >= add_ticks(before, t0);
+      const int first = second ? add_ticks(before, t0) : before;
+      const SeqBounds sb = second ? mine[1] : mine[0];
+      if (lane == src) x = stream_snap(stream_unit<kForm, kWide>(a, sb, first, at, ppu), at, a.min_piece);
+      x = __shfl_sync(0xffffffffu, x, src);
+      if (k == 0) {
+        sh.seq = __shfl_sync(0xffffffffu, 2 * lane + (second ? 1 : 0), src);
+        sh.seq_first = __shfl_sync(0xffffffffu, first, src);
+      }
+    }
+    if (k == 0) sh.x = x; else sh.end = x;
+  }
+  return sh;
+}
+
+// The same for any number of sequences, by the whole block; scratch: an int per
+// warp and 6 ints of shared memory.
+template <int kForm, bool kWide>
+__device__ __forceinline__ StreamShare stream_share_block(const AttnKernelArgs& a, int ppu, int* scratch) {
+  const int per = (a.num_seqs + kAttnThreads - 1) / kAttnThreads;
+  const int s0 = min(static_cast<int>(threadIdx.x) * per, a.num_seqs), s1 = min(s0 + per, a.num_seqs);
+  int ticks = 0;
+  for (int b = s0; b < s1; ++b) ticks = add_ticks(ticks, seq_ticks_clipped<kForm, kWide>(a, seq_bounds<kForm>(a, b), ppu));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = ticks;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum = add_ticks(sum, y);
   }
   if (lane == 31) scratch[warp] = sum;
+  int before = __shfl_up_sync(0xffffffffu, sum, 1);
+  if (lane == 0) before = 0;
   __syncthreads();
-  long long before = sum - ticks, all = 0;
-#pragma unroll
+  int total = 0;
   for (int w = 0; w < kAttnThreads / 32; ++w) {
-    if (w < warp) before += scratch[w];
-    all += scratch[w];
+    if (w < warp) before = add_ticks(before, scratch[w]);
+    total = add_ticks(total, scratch[w]);
   }
-  // The host has bounded the ticks of sequences that do not overlap; of others the rest is dropped.
-  const int total = static_cast<int>(min(all, 0x7fffffffll));
   StreamShare sh;
-  sh.ctas = max(1, min(static_cast<int>(gridDim.x), total / kStreamMinTicks));
-  sh.base = total / sh.ctas;
-  sh.extra = total - sh.base * sh.ctas;
-  int* out = reinterpret_cast<int*>(scratch + kAttnThreads / 32);  // (snapped tick, sequence, its first tick) of both ends
-#pragma unroll
+  sh.divide(total);
+  int* out = scratch + kAttnThreads / 32;  // (snapped tick, sequence, its first tick) of both ends
+#pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     const int at = sh.raw(min(static_cast<int>(blockIdx.x) + k, sh.ctas));
     if (threadIdx.x == 0 && at >= total) {
@@ -430,18 +485,17 @@ __device__ __forceinline__ StreamShare stream_share(const AttnKernelArgs& a, con
       out[3 * k + 1] = a.num_seqs;
       out[3 * k + 2] = total;
     }
-    if (at < total && at >= before && at < before + ticks) {
-      long long first = before;
-      int b = s0;
-      SeqBounds sb = per == 1 ? mine : seq_bounds<kForm>(a, b);
+    if (at < total && at >= before && at < add_ticks(before, ticks)) {
+      int first = before, b = s0;
+      SeqBounds sb = seq_bounds<kForm>(a, b);
       for (; b + 1 < s1; sb = seq_bounds<kForm>(a, ++b)) {
-        const long long t = seq_ticks<kForm, kWide>(a, sb, ppu);
-        if (at < first + t) break;
-        first += t;
+        const int t = add_ticks(first, seq_ticks_clipped<kForm, kWide>(a, sb, ppu));
+        if (at < t) break;
+        first = t;
       }
-      out[3 * k] = stream_snap(stream_unit<kForm, kWide>(a, sb, static_cast<int>(first), at, ppu), at);
+      out[3 * k] = stream_snap(stream_unit<kForm, kWide>(a, sb, first, at, ppu), at, a.min_piece);
       out[3 * k + 1] = b;
-      out[3 * k + 2] = static_cast<int>(first);
+      out[3 * k + 2] = first;
     }
   }
   __syncthreads();
@@ -516,8 +570,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int lane = threadIdx.x % 32;
   const int P = a.pos_per_tile;
   const int ppu = kTilesPerUnit * P;
-  SeqBounds my_seq{};  // streamed work: loaded here, used after the set-up
-  if (kStreamed && static_cast<int>(threadIdx.x) < a.num_seqs) my_seq = seq_bounds<kForm>(a, threadIdx.x);
+  SeqBounds my_seqs[2] = {};  // streamed work, producer warp: loaded here, used after the set-up
+  if (kStreamed && warp == 0 && a.num_seqs <= kStreamWarpSeqs) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (2 * lane + k < a.num_seqs) my_seqs[k] = seq_bounds<kForm>(a, 2 * lane + k);
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(bar(BAR_Q_FULL), 1);
@@ -560,10 +618,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     fence_proxy_async_smem();
   }
-  // Streamed work: this CTA's share (the unit ring's memory serves as scratch).
+  // Streamed work, many sequences: this CTA's share (the unit ring's memory serves as scratch).
   StreamShare share{};
-  if (kStreamed)
-    share = stream_share<kForm, kWide>(a, my_seq, ppu, reinterpret_cast<long long*>(smem + kSmBar + kSmRing));
+  if (kStreamed && a.num_seqs > kStreamWarpSeqs)
+    share = stream_share_block<kForm, kWide>(a, ppu, reinterpret_cast<int*>(smem + kSmBar + kSmRing));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -611,20 +669,32 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int my_slice = lane & 7;
       int4 meta = make_int4(0, 0, 0, 0);
       if (kStreamed && lane == 0) a.stream_meta[blockIdx.x] = meta;  // also when the loop below gives up early
-      if (kStreamed && static_cast<int>(blockIdx.x) >= share.ctas) share.end = share.x;
+      SeqBounds seq_b{};        // streamed: bounds and ticks of sequence share.seq
+      int seq_end = 0;
+      if (kStreamed) {
+        if (a.num_seqs <= kStreamWarpSeqs) share = stream_share_warp<kForm, kWide>(a, my_seqs, ppu);
+        if (static_cast<int>(blockIdx.x) >= share.ctas) share.end = share.x;
+        if (share.x < share.end) {
+          seq_b = seq_bounds<kForm>(a, share.seq);
+          seq_end = add_ticks(share.seq_first, seq_ticks_clipped<kForm, kWide>(a, seq_b, ppu));
+        }
+      }
       for (int it = 0;; ++it) {
         UnitEntry e{};
         if (kStreamed) {
           e.valid = share.x < share.end;
           while (e.valid) {
-            const SeqBounds sb = seq_bounds<kForm>(a, share.seq);
-            const long long ticks = seq_ticks<kForm, kWide>(a, sb, ppu);
-            if (share.x >= share.seq_first + ticks) {  // the sequence's units are done (or it has none)
-              share.seq_first += static_cast<int>(ticks);
-              if (++share.seq >= a.num_seqs) e.valid = 0;
+            if (share.x >= seq_end) {  // the sequence's units are done (or it has none)
+              share.seq_first = seq_end;
+              if (++share.seq >= a.num_seqs) {
+                e.valid = 0;
+              } else {
+                seq_b = seq_bounds<kForm>(a, share.seq);
+                seq_end = add_ticks(seq_end, seq_ticks_clipped<kForm, kWide>(a, seq_b, ppu));
+              }
               continue;
             }
-            const StreamUnit u = stream_unit<kForm, kWide>(a, sb, share.seq_first, share.x, ppu);
+            const StreamUnit u = stream_unit<kForm, kWide>(a, seq_b, share.seq_first, share.x, ppu);
             const int unit_end = u.first + u.ticks();
             const int piece_end = min(share.end, unit_end);
             const bool from_start = share.x == u.first, to_end = piece_end == unit_end;
@@ -635,16 +705,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             e.split = from_start ? 0 : (share.x - u.first - kStreamOverhead) >> (u.weight - 1);
             e.nsplit = to_end ? u.tiles : (piece_end - u.first - kStreamOverhead) >> (u.weight - 1);
             e.slot = from_start && to_end ? -1 : 2 * static_cast<int>(blockIdx.x) + (from_start ? 1 : 0);
-            e.q_begin = sb.q_begin;
-            e.q_end = sb.q_end;
-            e.seq_len = sb.seq_len;
-            e.k_begin = sb.k_begin;
+            e.q_begin = seq_b.q_begin;
+            e.q_end = seq_b.q_end;
+            e.seq_len = seq_b.seq_len;
+            e.k_begin = seq_b.k_begin;
             if (from_start && !to_end) {
               // The CTAs behind this one whose share begins inside the unit hold its other pieces.
               int pieces = 1;
               for (int i0 = static_cast<int>(blockIdx.x) + 1; i0 < share.ctas; i0 += 32) {
                 const int i = i0 + lane, x = i < share.ctas ? share.raw(i) : unit_end;
-                const unsigned in = __ballot_sync(0xffffffffu, x < unit_end && stream_snap(u, x) < unit_end);
+                const unsigned in = __ballot_sync(0xffffffffu, x < unit_end && stream_snap(u, x, a.min_piece) < unit_end);
                 pieces += __popc(in);
                 if (in != 0xffffffffu) break;
               }
@@ -1335,7 +1405,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           a.l_split[rowi] = l;
         }
       }
-#pragma unroll
+      constexpr int kEpilogueUnroll = kStreamed ? 1 : 8;
+#pragma unroll kEpilogueUnroll
       for (int c4 = 0; c4 < (kWide ? 8 : kNarrow ? 2 : 4); ++c4) {
         if (c4 * 32 >= a.head_dim) break;  // warp-uniform: only the row's real columns
         if (kStreamed && dual && (c4 >= (kNarrow ? 1 : 2)) != (t == 1)) continue;  // the other group's half
@@ -1376,7 +1447,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           uint32_t w[16];
 #pragma unroll
           for (int v = 0; v < 16; ++v) w[v] = Pack2<T>::pack(__uint_as_float(o[2 * v]), __uint_as_float(o[2 * v + 1]));
-          if (kStreamed && a.wide_out) {  // whole 32-byte sectors
+          if (kForm != kFormPaged && a.wide_out) {  // whole 32-byte sectors
             st_global_v8(dst + c4 * 32, w);
             st_global_v8(dst + c4 * 32 + 16, w + 8);
           } else {

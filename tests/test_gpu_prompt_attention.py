@@ -156,6 +156,23 @@ def test_large_scores_do_not_overflow():
     _check(out, q, k, v, ql, ql, 0.125, True)
 
 
+@pytest.mark.parametrize("n", [64, 65, 150])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_short_sequences(n, causal):
+    """Up to 64 sequences one warp divides the work, above that the block; one KV head keeps the batch small."""
+    ql = [(7 * i) % 11 for i in range(n)]
+    _run(ql, ql, 2, 1, 64, torch.bfloat16, causal, seed=n)
+
+
+@pytest.mark.parametrize("hint", [0, 1, 700, 1 << 20])
+def test_a_wrong_bound_of_the_longest_sequence_costs_time_only(hint):
+    ql, kl = [5, 40, 0, 9], [1500, 40, 3, 700]
+    q, k, v = _inputs(ql, kl, 4, 1, 128, torch.bfloat16, 2)
+    out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
+    prompt_attention(q.cuda(), k.cuda(), v.cuda(), out, _cu(ql).cuda(), 40, 0.1, cu_seqlens_k=_cu(kl).cuda(), max_seqlen_k=hint)
+    _check(out, q, k, v, ql, kl, 0.1, True)
+
+
 def test_lengths_past_the_tensors_stay_in_bounds():
     """cu_seqlens that name rows the tensors do not have are clipped; rows behind stay as they were."""
     q, k, v = (t.cuda() for t in _inputs([64], [64], 4, 2, 64, torch.bfloat16, 6))

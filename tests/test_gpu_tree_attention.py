@@ -108,6 +108,19 @@ def test_long_contexts_are_split_and_combined():
         b.check(b.run(), tag=f"{ctx} {n} {dim}")
 
 
+@pytest.mark.parametrize("n", [64, 65, 400])
+def test_many_sequences(n):
+    r = random.Random(n)
+    b = Batch([r.randrange(40) for _ in range(n)], [r.randrange(6) for _ in range(n)], hq=4, hkv=2, dim=64, seed=n)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("hint", [1, 600, 1 << 20])
+def test_a_wrong_bound_of_the_longest_sequence_costs_time_only(hint):
+    b = Batch([2100, 33], [9, 40], hq=8, hkv=1, seed=3)
+    b.check(b.run(max_seqlen_k=hint))
+
+
 def test_masks_that_leave_rows_empty_and_unseen_garbage():
     """A row that sees nothing is 0; K/V of tokens past the length may be NaN; so may tail pages."""
     b = Batch([0, 40, 0], [20, 9, 3], seed=3)
