@@ -82,10 +82,10 @@ int read_table(const B200SeqTable* p, b200::SeqTable* t) {
   return B200_OK;
 }
 
-// CTAs for `warps` warps of work, at most what fills the GPU.
-dim3 warp_grid(int64_t warps) {
-  const int64_t per = b200::kPageThreads / 32;
-  return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>((warps + per - 1) / per, (int64_t)sm_count() * 8)));
+// CTAs for `warps` warps of work in each of `layers` grid rows, at most what fills the GPU.
+dim3 warp_grid(int64_t warps, int layers = 1) {
+  const int64_t per = b200::kPageThreads / 32, most = ((int64_t)sm_count() * 8 + layers - 1) / layers;
+  return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>((warps + per - 1) / per, most)), (unsigned)layers);
 }
 
 template <typename... KArgs, typename... Args>
@@ -170,9 +170,8 @@ int b200_fork_sequences(const B200PageCaches* caches, const B200SeqTable* table,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   b200::fork_plan_kernel<0><<<1, b200::kForkThreads, 0, s>>>(a);
   if (int r = check_launch("fork_plan_kernel")) return r;
-  const int64_t copy_warps =
-      (int64_t)num_entries * ((a.t.block_size + b200::kForkToks - 1) / b200::kForkToks) * c.shape.num_caches;
-  const dim3 grid = warp_grid(std::max<int64_t>(copy_warps, (int64_t)num_entries * ((a.t.cols + 31) / 32)));
+  const int64_t parts = (a.t.block_size + b200::kForkToks - 1) / b200::kForkToks;
+  const dim3 grid = warp_grid(num_entries * std::max<int64_t>(parts, (a.t.cols + 31) / 32), c.shape.num_caches + 1);
   return c.wide ? launch_after("fork_apply_kernel", b200::fork_apply_kernel<uint4>, grid, s, c.set, a)
                 : launch_after("fork_apply_kernel", b200::fork_apply_kernel<uint32_t>, grid, s, c.set, a);
 }
@@ -216,7 +215,7 @@ int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable* table, 
   a.most = most;
   a.idx_i64 = index_dtype == B200_DTYPE_I64;
   const int pieces = c.shape.seg_bytes * c.shape.segs / (c.wide ? 16 : 4);
-  const dim3 grid = warp_grid((int64_t)a.num_seqs * ((pieces + 31) / 32) * c.shape.num_caches);
+  const dim3 grid = warp_grid((int64_t)a.num_seqs * ((pieces + 31) / 32), c.shape.num_caches);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c.wide) b200::keep_accepted_kernel<uint4><<<grid, b200::kPageThreads, 0, s>>>(c.set, a);
   else b200::keep_accepted_kernel<uint32_t><<<grid, b200::kPageThreads, 0, s>>>(c.set, a);
