@@ -140,14 +140,35 @@ struct FormLayout {
   size_t total;
 };
 
+// Whole units that the batch is sure to have: as many as its query rows fill, and one
+// for each sequence at least.
+inline int64_t sure_units(int64_t total_q, int num_seqs, int ppu, int hkv) {
+  return std::max<int64_t>((total_q + ppu - 1) / ppu, std::min<int64_t>(num_seqs, total_q)) * hkv;
+}
+
 // Draft trees are always streamed.  Prompts are where whole units would leave SMs
-// idle: fewer units than SMs, or few rounds of long ones.  Elsewhere the list wins:
-// its dynamic claims balance better, and it writes no partials (33 sequences of up
-// to 517 tokens x 12 heads: 52 us listed, 74 us streamed).
+// idle: fewer units than SMs, or few rounds of long units that are all alike
+// (bidirectional, or queries over longer prefixes) and fill the last round badly.
+// Elsewhere the list wins, whose dynamic claims balance the unequal units of causal
+// prompts and which writes no partials.  Listed / streamed, 16 query and 2 KV heads
+// of 128: 2 x 8192 causal (6.9 rounds) 475 / 593 us, 1 x 4096 causal 82 / 110 us, 33
+// sequences of up to 517 x 12 heads of 64 bidirectional 51 / 74 us; 8 x 512 over 8192
+// (1.7 rounds) 311 / 293 us, 4 x 2048 over 14000 (3.5) 1027 / 943 us, 2 x 4096 x 12
+// heads bidirectional (2.6) 206 / 196 us, but 16 x 1024 over 4096 (6.9) 552 / 599 us.
 constexpr int kStreamRounds = 8;
 constexpr int kStreamLongTiles = 32;
 
-inline FormLayout form_layout(bool tree, int64_t total_q, int num_seqs, int hq, int hkv, int head_dim,
+inline bool stream_prompt(int64_t total_q, int64_t total_k, int num_seqs, int ppu, int hkv, int max_seqlen_k, bool causal,
+                          int sms) {
+  const int64_t units = sure_units(total_q, num_seqs, ppu, hkv);
+  if (units < sms) return true;
+  const bool alike = !causal || total_k >= 2 * total_q;
+  const int64_t rounds = (units + sms - 1) / sms;
+  return alike && rounds <= kStreamRounds && max_seqlen_k >= kStreamLongTiles * b200::kAttnTileN &&
+         10 * rounds * sms > 11 * units;  // the last round leaves more than a tenth idle
+}
+
+inline FormLayout form_layout(bool streamed, int64_t total_q, int num_seqs, int hq, int hkv, int head_dim,
                               int max_seqlen_k, int sms) {
   FormLayout w{};
   const int group = hq / hkv;
@@ -157,9 +178,7 @@ inline FormLayout form_layout(bool tree, int64_t total_q, int num_seqs, int hq, 
   w.capacity = w.qunits_ub * hkv;
   const int64_t tiles = std::max(max_seqlen_k, 0) / b200::kAttnTileN + 1;
   const int64_t ticks = w.capacity * (b200::kStreamOverhead + 2 * tiles);
-  const int64_t units_lb =
-      std::max<int64_t>((total_q + w.ppu - 1) / w.ppu, std::min<int64_t>(num_seqs, total_q)) * hkv;
-  w.streamed = tree || units_lb < sms || (units_lb < (int64_t)kStreamRounds * sms && tiles >= kStreamLongTiles);
+  w.streamed = streamed;
   w.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(w.streamed ? ticks / b200::kStreamMinTicks : w.capacity, sms));
   // No unit as long as two pieces (by the caller's bound): none is shared, and there
   // is nothing to join.

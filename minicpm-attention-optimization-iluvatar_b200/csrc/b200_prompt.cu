@@ -76,7 +76,10 @@ int b200_prompt_attn_fwd(const B200PromptAttnParams* p, void* stream) {
   a.full = p->causal ? 0 : 1;
   a.scale_log2 = static_cast<float>(static_cast<double>(p->softmax_scale) * 1.4426950408889634);
   const int sms = sm_count();
-  const FormLayout w = form_layout(false, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim,
+  const int ppu = ppt * (p->head_dim == 256 ? 1 : b200::kAttnTilesPerUnit);
+  const bool streamed = stream_prompt(p->total_q, p->total_k, p->num_seqs, ppu, p->num_kv_heads, p->max_seqlen_k,
+                                      p->causal != 0, sms);
+  const FormLayout w = form_layout(streamed, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim,
                                    p->max_seqlen_k, sms);
   const int64_t max_tiles = (int64_t)p->total_k / b200::kAttnTileN + 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

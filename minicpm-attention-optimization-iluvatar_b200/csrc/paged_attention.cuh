@@ -313,7 +313,10 @@ __device__ __forceinline__ UnitGeom piece_geometry(int q_begin, int q_end, int s
 }
 
 // Streamed work.  Ticks of a unit: kStreamOverhead + k tiles, k = 2 where two query
-// tiles share the KV tiles, else 1 (a tick is about a microsecond).
+// tiles share the KV tiles, else 1 (a tick is about a microsecond).  Measured, one
+// draft of 16 nodes over 4096 keys / four prompts of up to 131 tokens: a share of 3
+// ticks at least 18.5 / 12.7 us, 4 ticks 19.8 / 14.7, 6 ticks 22 / 18.7; an overhead
+// of 4 ticks 19.1 / 12.7.
 constexpr int kStreamOverhead = 2;
 constexpr int kStreamMinTicks = 3;  // a CTA's share at least
 constexpr int kStreamMinTiles = 2;  // KV tiles of a piece at least: fewer do not pay for its partial

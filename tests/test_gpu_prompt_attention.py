@@ -156,6 +156,21 @@ def test_large_scores_do_not_overflow():
     _check(out, q, k, v, ql, ql, 0.125, True)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_batches_that_fill_the_gpu(dim, dtype, causal):
+    """More whole units than SMs: the schedule kernel's list."""
+    ql = [(37 * i) % 300 for i in range(24)]
+    _run(ql, ql, 16, 8, dim, dtype, causal, seed=dim)
+
+
+def test_few_rounds_of_long_units_are_shared():
+    """150 equal units on 148 SMs: streamed although there are more units than SMs."""
+    ql, kl = [9] * 75, [4100] * 75
+    _run(ql, kl, 4, 2, 64, torch.bfloat16, True, seed=1)
+
+
 @pytest.mark.parametrize("n", [64, 65, 150])
 @pytest.mark.parametrize("causal", [True, False])
 def test_many_short_sequences(n, causal):
