@@ -16,24 +16,31 @@ cudaError_t tree_device_error(unsigned int* code) {
 
 namespace {
 
+// Keys per TMA box: the largest power of two, 16 to 128, that divides the page.
+int slice_keys(int block_size) {
+  int s = 16;
+  while (s < b200::kAttnTileN && block_size % (2 * s) == 0) s *= 2;
+  return s;
+}
+
 // K/V maps of a paged cache [num_blocks, block_size, KH, D]: one 5-D map per KV
-// head (16-key slices of both halves, 4 KB a box) for up to kMaxHeadMaps heads,
-// else one 4-D map (2 KB a box); the layouts are those of the paged form.
+// head (a slice with both halves, 4 KB a box at 16 keys) for up to kMaxHeadMaps
+// heads, else one 4-D map (one half a box); the layouts are those of the paged form.
 int encode_pages(const B200TreeAttnParams* p, const void* base, int64_t sb, int64_t st, int64_t sh, bool head_maps,
-                 CUtensorMap* maps, const char* what) {
+                 int slice, CUtensorMap* maps, const char* what) {
   if (p->num_blocks == 1) sb = (int64_t)p->block_size * st;
   if (p->num_kv_heads == 1) sh = p->head_dim;
   if (!head_maps) {
     const cuuint64_t dims[4] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->block_size, (cuuint64_t)p->num_kv_heads,
                                 (cuuint64_t)p->num_blocks};
     const cuuint64_t strides[3] = {(cuuint64_t)(st * 2), (cuuint64_t)(sh * 2), (cuuint64_t)(sb * 2)};
-    const cuuint32_t box[4] = {64, 16, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)slice, 1, 1};
     return encode_map(&maps[0], map_type(p->dtype), 4, base, dims, strides, box, what);
   }
   const cuuint64_t dims[5] = {64, 8, (cuuint64_t)(p->head_dim / 64), (cuuint64_t)(p->block_size / 8),
                               (cuuint64_t)p->num_blocks};
   const cuuint64_t strides[4] = {(cuuint64_t)(st * 2), 128, (cuuint64_t)(8 * st * 2), (cuuint64_t)(sb * 2)};
-  const cuuint32_t box[5] = {64, 8, (cuuint32_t)std::min(2, p->head_dim / 64), 2, 1};
+  const cuuint32_t box[5] = {64, 8, (cuuint32_t)std::min(2, p->head_dim / 64), (cuuint32_t)(slice / 8), 1};
   for (int h = 0; h < p->num_kv_heads; ++h)
     if (int r = encode_map(&maps[h], map_type(p->dtype), 5, static_cast<const uint8_t*>(base) + (int64_t)h * sh * 2, dims,
                            strides, box, what))
@@ -68,9 +75,10 @@ int b200_tree_attn_fwd(const B200TreeAttnParams* p, void* stream) {
                           p->q_stride_h, group, ppt, "q"))
     return r;
   f.head_maps = p->num_kv_heads <= b200::kMaxHeadMaps;
-  if (int r = encode_pages(p, p->k, p->k_stride_block, p->k_stride_tok, p->k_stride_head, f.head_maps, f.maps.k, "k"))
+  const int slice = slice_keys(p->block_size);
+  if (int r = encode_pages(p, p->k, p->k_stride_block, p->k_stride_tok, p->k_stride_head, f.head_maps, slice, f.maps.k, "k"))
     return r;
-  if (int r = encode_pages(p, p->v, p->v_stride_block, p->v_stride_tok, p->v_stride_head, f.head_maps, f.maps.v, "v"))
+  if (int r = encode_pages(p, p->v, p->v_stride_block, p->v_stride_tok, p->v_stride_head, f.head_maps, slice, f.maps.v, "v"))
     return r;
   f.dtype = p->dtype;
   f.num_seqs = p->num_seqs;
@@ -93,6 +101,7 @@ int b200_tree_attn_fwd(const B200TreeAttnParams* p, void* stream) {
   a.num_q_heads = p->num_q_heads;
   a.group = group;
   a.block_size = p->block_size;
+  a.slice = slice;
   a.num_blocks = p->num_blocks;
   a.head_dim = p->head_dim;
   a.tree_mask = static_cast<const uint8_t*>(p->tree_mask);

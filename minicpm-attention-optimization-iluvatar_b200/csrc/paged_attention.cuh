@@ -200,6 +200,7 @@ struct AttnKernelArgs {
   int total_k;
   int full;                  // every row's keys end at L (bidirectional, or masked by the tree)
   int wide_out;              // rows of out are 32-byte aligned
+  int slice;                 // kFormTree: keys per page slice (16, 32, 64 or 128, a divisor of the page size)
   int min_piece;             // streamed: KV tiles of a piece at least; no unit is shared where none has twice that
   int num_seqs, num_kv_heads;
   int4* stream_meta;         // [grid]: sequence, query unit, KV head, pieces of the unit that CTA i begins and does not end (0: none)
@@ -216,6 +217,9 @@ struct KvHeadMaps {
   CUtensorMap k[kMaxHeadMaps];
   CUtensorMap v[kMaxHeadMaps];
 };
+
+// End of the slice that holds key n - 1 (slices are powers of two).
+__device__ __forceinline__ int slice_up(int n, int slice) { return (n + slice - 1) & -slice; }
 
 // Shared-memory offset of the 16-byte piece `chunk` of row r (a key) of half h
 // in one K/V ring slot.  Per-head maps: 8-key groups of 2 KB, each holding both
@@ -669,7 +673,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       int* claim = const_cast<int*>(a.unit_count) + 1;  // reset to 0 by the schedule kernel
       int issued = 0;   // K/V ring fills so far
       int q_loads = 0;  // Q loads so far
-      const int my_slice = lane & 7;
+      // Keys per page slice and slices per tile: one TMA box (per half) brings a slice.
+      // Pages of 32 keys or more take larger boxes, whose per-box cost in the TMA unit
+      // weighs less (see KvHeadMaps).
+      const int slice = kForm == kFormTree ? a.slice : kAttnSlice;
+      const int slices = kAttnTileN / slice;
+      const int my_slice = lane & (slices - 1);
       int4 meta = make_int4(0, 0, 0, 0);
       if (kStreamed && lane == 0) a.stream_meta[blockIdx.x] = meta;  // also when the loop below gives up early
       SeqBounds seq_b{};        // streamed: bounds and ticks of sequence share.seq
@@ -802,7 +811,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         ++q_loads;
         const int64_t bt_row = static_cast<int64_t>(e.seq) * a.bt_stride;
         auto lookup = [&](int j, int& pg, int& of) {
-          const int pos = ug.kv_lo + j * kAttnTileN + my_slice * kAttnSlice;
+          const int pos = ug.kv_lo + j * kAttnTileN + my_slice * slice;
           const int lp = pos / a.block_size;
           of = pos - lp * a.block_size;
           const int lpc = min(lp, a.bt_cols - 1);
@@ -838,7 +847,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             if (j + 1 < n_tiles) lookup(j + 1, pg_nxt, of_nxt);
           }
           // 4-D maps: lanes 0..15 issue half lane & 1 of slice (lane >> 1); head_dim 64: lane c < 8 slice c.
-          const int c = kNarrow ? (lane & 7) : ((lane >> 1) & 7);
+          const int c = (kNarrow ? lane : lane >> 1) & (slices - 1);
           const bool behind = dual && is_v && j + 1 < n_tiles;  // V_j comes after K_{j + 1}
           const int pg = behind ? pg_prev : pg_cur, of = behind ? of_prev : of_cur;
           const int page = kHeadMaps ? pg : __shfl_sync(0xffffffffu, pg, c);
@@ -858,15 +867,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                           bar(BAR_KV_FULL + slot), lane * 64 + hi * 128, e.kvh, e.k_begin + ug.kv_lo + j * kAttnTileN);
           } else if (kHeadMaps) {
             // lane c < 8 issues slice c (its own lookup): 16 keys x both halves.
-            if (lane < 8) {
+            if (lane < slices) {
               const CUtensorMap* map = is_v ? &maps.v[e.kvh] : &maps.k[e.kvh];
-              tma_load_5d(sbase + kSmKV + slot * 32768 + lane * (kNarrow ? 2048 : 4096), map,
+              tma_load_5d(sbase + kSmKV + slot * 32768 + lane * slice * (kNarrow ? 128 : 256), map,
                           bar(BAR_KV_FULL + slot), 0, 0, 2 * hi, off >> 3, page);
             }
-          } else if (lane < (kNarrow ? 8 : 16)) {
+          } else if (lane < (kNarrow ? slices : 2 * slices)) {
             const int half = kNarrow ? 0 : (lane & 1);
             const CUtensorMap* map = is_v ? &maps.v[0] : &maps.k[0];
-            tma_load_4d(sbase + kSmKV + slot * 32768 + half * 16384 + c * 2048, map, bar(BAR_KV_FULL + slot),
+            tma_load_4d(sbase + kSmKV + slot * 32768 + half * 16384 + c * slice * 128, map, bar(BAR_KV_FULL + slot),
                         half * 64 + hi * 128, off, e.kvh, page);
           }
           ++issued;
@@ -1139,7 +1148,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int v_tail_from = max(ug.seq_len - last_start, 0);
       const int v_tail_to = form_rows(kForm)
                                 ? kAttnTileN
-                                : min(((ug.kv_hi + kAttnSlice - 1) / kAttnSlice) * kAttnSlice - last_start, kAttnTileN);
+                                : min(slice_up(ug.kv_hi, kForm == kFormTree ? a.slice : kAttnSlice) - last_start, kAttnTileN);
 
       float m_used = -INFINITY;  // running maximum in scaled base-2 units
       float l = 0.f;
