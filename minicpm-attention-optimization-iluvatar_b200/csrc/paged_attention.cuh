@@ -248,23 +248,29 @@ struct UnitGeom {
 struct SeqBounds {
   int q_begin, q_end, seq_len, k_begin;
 };
+// Element i of an int32 / int64 array, clipped to [lo, hi].
+__device__ __forceinline__ int load_clipped(const void* p, int64_t i, int is_i64, int lo, int64_t hi) {
+  const int64_t v = is_i64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int*>(p)[i];
+  return static_cast<int>(min(max(v, static_cast<int64_t>(lo)), hi));
+}
 template <int kForm, typename Args>
 __device__ __forceinline__ SeqBounds seq_bounds(const Args& a, int b) {
   SeqBounds s{};
-  s.q_begin = load_index(a.cu_q, b, a.len_i64);
-  s.q_end = load_index(a.cu_q, b + 1, a.len_i64);
-  if (kForm != kFormPaged) {
-    s.q_begin = min(max(s.q_begin, 0), a.total_q);
-    s.q_end = min(max(s.q_end, s.q_begin), a.total_q);
-  }
-  if (form_rows(kForm)) {
-    s.k_begin = min(max(load_index(a.cu_k, b, a.len_i64), 0), a.total_k);
-    s.seq_len = min(max(load_index(a.cu_k, b + 1, a.len_i64), s.k_begin), a.total_k) - s.k_begin;
-  } else {
+  if (kForm == kFormPaged) {
+    s.q_begin = load_index(a.cu_q, b, a.len_i64);
+    s.q_end = load_index(a.cu_q, b + 1, a.len_i64);
     s.seq_len = load_index(a.seqused, b, a.len_i64);
+    return s;
+  }
+  s.q_begin = load_clipped(a.cu_q, b, a.len_i64, 0, a.total_q);
+  s.q_end = load_clipped(a.cu_q, b + 1, a.len_i64, s.q_begin, a.total_q);
+  if (form_rows(kForm)) {
+    s.k_begin = load_clipped(a.cu_k, b, a.len_i64, 0, a.total_k);
+    s.seq_len = load_clipped(a.cu_k, b + 1, a.len_i64, s.k_begin, a.total_k) - s.k_begin;
+  } else {
     // A table row holds bt_cols pages; keys past them do not exist.
-    if (kForm == kFormTree)
-      s.seq_len = static_cast<int>(min(static_cast<int64_t>(max(s.seq_len, 0)), static_cast<int64_t>(a.bt_cols) * a.block_size));
+    const int64_t room = static_cast<int64_t>(a.bt_cols) * a.block_size;
+    s.seq_len = load_clipped(a.seqused, b, a.len_i64, 0, min(room, static_cast<int64_t>(0x7fffff00)));
   }
   return s;
 }
@@ -815,7 +821,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const int lp = pos / a.block_size;
           of = pos - lp * a.block_size;
           const int lpc = min(lp, a.bt_cols - 1);
-          const int v = load_index(a.block_table, bt_row + lpc, a.bt_i64);
+          // (an int64 id past int32 must not come back in range)
+          const int v = kForm == kFormPaged ? load_index(a.block_table, bt_row + lpc, a.bt_i64)
+                                            : load_clipped(a.block_table, bt_row + lpc, a.bt_i64, -1, a.num_blocks);
           pg = (pos < ug.kv_hi && lp < a.bt_cols) ? v : a.num_blocks;
         };
         int pg_cur = 0, of_cur = 0, pg_nxt = a.num_blocks, of_nxt = 0, pg_prev = 0, of_prev = 0;

@@ -233,8 +233,8 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
     counts = _indices("num_accepted", num_accepted, dev)
     if counts.shape[0] != accepted.shape[0] or counts.dtype != accepted.dtype:
         raise ValueError("num_accepted must hold one count per row, in the dtype of accepted")
-    if context_lens.numel() and context_lens.data_ptr() == seq_lens.data_ptr():
-        raise ValueError("seq_lens may not be context_lens")
+    if abs(context_lens.data_ptr() - seq_lens.data_ptr()) < seq_lens.numel() * seq_lens.element_size():
+        raise ValueError("seq_lens may not be (or overlap) context_lens")
     _cuda(dev, "keep_accepted_tokens")
     if accepted.shape[1] and (accepted.stride(1) != 1 or accepted.stride(0) < accepted.shape[1]):
         accepted = accepted.contiguous()

@@ -93,6 +93,18 @@ def test_page_sizes(page):
     b.check(b.run())
 
 
+@pytest.mark.parametrize("page", [32, 64, 128, 384])
+@pytest.mark.parametrize("dim,hq,hkv", [(64, 9, 9), (128, 12, 12), (256, 10, 10), (64, 4, 2), (256, 4, 2)])
+def test_larger_slices(page, dim, hq, hkv):
+    """Pages of 32 keys and more come in larger boxes, through one map per head and through one for all."""
+    b = Batch([129, 5, 600], [9, 21, 3], hq=hq, hkv=hkv, dim=dim, page=page, seed=page + dim)
+    cache = b.cache.clone()
+    for row, L in enumerate(b.lens):  # the rest of every last page may hold anything
+        if L % page:
+            cache[int(b.table[row, L // page]), :, L % page:] = float("nan")
+    b.check(b.run(cache=cache.cuda()))
+
+
 @pytest.mark.parametrize("nodes", [1, 2, 15, 16, 17, 63, 64, 65, 128, 200])
 @pytest.mark.parametrize("hq", [2, 16])
 def test_trees_around_the_tiles(nodes, hq):
@@ -189,9 +201,15 @@ def test_bad_pages_and_lengths_stay_in_bounds():
     table[0, 1], table[0, 2] = 1 << 30, -7
     out = b.run(block_table=table.cuda())
     assert torch.isfinite(out.float()).all()  # such a page reads as zeros
+    far = table.long()
+    far[0, 1], far[0, 2] = (1 << 32) + 1, -(1 << 32)
+    assert torch.equal(b.run(block_table=far.cuda()), out)
     want = b.run()
     out = b.run(seqused_k=torch.tensor([1 << 30], dtype=torch.int32).cuda())  # clipped to the table's pages
     assert torch.isfinite(out.float()).all() and out.shape == want.shape
+    wide = dict(cu_seqlens_q=b.cu.long().cuda())
+    far = b.run(seqused_k=torch.tensor([(1 << 32) + 108]).cuda(), **wide)  # not 108
+    assert torch.equal(far, out)
     out = b.run(seqused_k=torch.tensor([-4], dtype=torch.int32).cuda())
     assert out.abs().max().item() == 0.0
     out = b.run(cu_seqlens_q=torch.tensor([0, 1 << 29], dtype=torch.int32).cuda())

@@ -174,7 +174,10 @@ def test_copy_free_and_keep_refusals():
 
     for over, msg in [(dict(context=ctx.long()), "must match seq_lens"), (dict(accepted=acc[:2]), "one row per row"),
                       (dict(counts=num.long()), "dtype of accepted"), (dict(counts=num[:2]), "one count per row"),
-                      (dict(lens=ctx), "may not be context_lens")]:
+                      (dict(lens=ctx), "context_lens"),
+                      (dict(context=torch.zeros(9, dtype=torch.int32)[1:4], lens=None), "context_lens")]:
+        if over.get("lens", 0) is None:  # two views of one buffer that overlap
+            over["lens"] = over["context"].as_strided((3,), (1,), 0)
         with pytest.raises(ValueError, match=msg):
             keep(**over)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
