@@ -300,6 +300,11 @@ def current_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+@functools.lru_cache(maxsize=256)
+def fork_workspace_bytes(num_entries: int, max_seqs: int) -> int:
+    return int(load().b200_fork_workspace_bytes(num_entries, max_seqs))
+
+
 _NO_SWITCH = contextlib.nullcontext()
 
 

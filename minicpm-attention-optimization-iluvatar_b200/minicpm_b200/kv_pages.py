@@ -93,26 +93,32 @@ def cache_layers(kv_caches: Caches) -> CacheLayers:
     return kv_caches if isinstance(kv_caches, CacheLayers) else CacheLayers(kv_caches)
 
 
-_INDEX_TYPES = (torch.int32, torch.int64)
+_INDEX_CODES = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
 
-def _indices(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if t.ndim != 1 or t.dtype not in _INDEX_TYPES:
+def _indices(name: str, t: torch.Tensor, device: torch.device) -> tuple[torch.Tensor, int, int]:
+    """``t`` (contiguous), its length and the code of its dtype."""
+    code = _INDEX_CODES.get(t.dtype)
+    if code is None or t.ndim != 1:
         raise ValueError(f"{name} must be a one-dimensional int32 or int64 tensor")
     if t.device != device:
         raise ValueError(f"{name} must be on the same device as the table or caches")
-    return t if t.is_contiguous() else t.contiguous()
+    return t if t.is_contiguous() else t.contiguous(), t.shape[0], code
 
 
 def _table(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: Optional[torch.Tensor], num_blocks: int,
-           block_size: int) -> "_lib.SeqTable":
-    if block_table.ndim != 2 or block_table.dtype not in _INDEX_TYPES or block_table.shape[1] == 0:
+           block_size: int) -> tuple["_lib.SeqTable", int, torch.device]:
+    """The table as the library takes it, its rows and its device."""
+    code, len_code = _INDEX_CODES.get(block_table.dtype), _INDEX_CODES.get(seq_lens.dtype)
+    if code is None or block_table.ndim != 2:
         raise ValueError("block_table must contain integer physical block ids, [max_seqs, max_pages]")
     rows, cols = block_table.shape
+    if cols == 0:
+        raise ValueError("block_table must contain integer physical block ids, [max_seqs, max_pages]")
     stride, step = block_table.stride()
     if step != 1 or (rows > 1 and stride < cols):
         raise ValueError("block_table is written in place: its rows must be contiguous and apart")
-    if seq_lens.ndim != 1 or seq_lens.shape[0] != rows or seq_lens.dtype not in _INDEX_TYPES:
+    if len_code is None or seq_lens.ndim != 1 or seq_lens.shape[0] != rows:
         raise ValueError("seq_lens must hold one int32 or int64 length per row of the block table")
     if not seq_lens.is_contiguous():
         raise ValueError("seq_lens is written in place: it must be contiguous")
@@ -121,21 +127,19 @@ def _table(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: Option
         raise ValueError("block_table and seq_lens must be on the same device")
     refs = None
     if ref_counts is not None:
-        if ref_counts.ndim != 1 or ref_counts.dtype != torch.int32 or ref_counts.shape[0] != num_blocks:
+        if ref_counts.ndim != 1 or ref_counts.dtype is not torch.int32 or ref_counts.shape[0] != num_blocks:
             raise ValueError("ref_counts must hold one int32 per page")
         if not ref_counts.is_contiguous() or ref_counts.device != dev:
             raise ValueError("ref_counts is written in place: contiguous, on the table's device")
         refs = ref_counts.data_ptr()
-    return _lib.SeqTable(block_table.data_ptr(), seq_lens.data_ptr(), refs, stride if rows > 1 else max(stride, cols), cols,
-                         rows, num_blocks, block_size, _lib.dtype_code(block_table.dtype), _lib.dtype_code(seq_lens.dtype))
+    table = _lib.SeqTable(block_table.data_ptr(), seq_lens.data_ptr(), refs, stride if rows > 1 else max(stride, cols), cols,
+                          rows, num_blocks, block_size, code, len_code)
+    return table, rows, dev
 
 
-def _same_device(layers: CacheLayers, dev: torch.device) -> None:
+def _on(layers: CacheLayers, dev: torch.device, what: str) -> None:
     if layers.device != dev:
         raise ValueError("the caches and the indices must be on the same device")
-
-
-def _cuda(dev: torch.device, what: str) -> None:
     if dev.type != "cuda":
         raise RuntimeError(f"{what} runs on CUDA tensors only (no CPU path)")
 
@@ -148,14 +152,15 @@ def copy_pages(kv_caches: Caches, src_pages: torch.Tensor, dst_pages: torch.Tens
     """
     layers = cache_layers(kv_caches)
     dev = layers.device
-    src, dst = _indices("src_pages", src_pages, dev), _indices("dst_pages", dst_pages, dev)
-    if src.shape != dst.shape or src.dtype != dst.dtype:
+    src, n, code = _indices("src_pages", src_pages, dev)
+    dst, n_dst, dst_code = _indices("dst_pages", dst_pages, dev)
+    if n != n_dst or code != dst_code:
         raise ValueError("src_pages and dst_pages must have one length and dtype")
-    _cuda(dev, "copy_pages")
+    _on(layers, dev, "copy_pages")
     lib = _lib.load()
     with _lib.on_device(dev):
-        _lib.check(lib.b200_copy_pages(layers._ref, src.data_ptr(), dst.data_ptr(), src.shape[0],
-                                       _lib.dtype_code(src.dtype), _lib.current_stream(dev)), "copy_pages")
+        _lib.check(lib.b200_copy_pages(layers._ref, src.data_ptr(), dst.data_ptr(), n, code, _lib.current_stream(dev)),
+                   "copy_pages")
 
 
 def fork_sequences(kv_caches: Caches, block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor,
@@ -169,25 +174,22 @@ def fork_sequences(kv_caches: Caches, block_table: torch.Tensor, seq_lens: torch
     that cannot be served leaves its child empty and is recorded.
     """
     layers = cache_layers(kv_caches)
-    dev = layers.device
-    table = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)
-    _same_device(layers, block_table.device)
+    table, rows, dev = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)
     if ref_counts is None:
         raise ValueError("fork_sequences needs ref_counts")
-    p, c = _indices("parents", parents, dev), _indices("children", children, dev)
-    if p.shape != c.shape or p.dtype != c.dtype:
+    p, n, code = _indices("parents", parents, dev)
+    c, n_children, c_code = _indices("children", children, dev)
+    if n != n_children or code != c_code:
         raise ValueError("parents and children must have one length and dtype")
-    _cuda(dev, "fork_sequences")
-    n = p.shape[0]
+    _on(layers, dev, "fork_sequences")
     if n == 0:
         return
     lib = _lib.load()
     with _lib.on_device(dev):
-        nbytes = lib.b200_fork_workspace_bytes(n, block_table.shape[0])
+        nbytes = _lib.fork_workspace_bytes(n, rows)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.check(lib.b200_fork_sequences(layers._ref, ctypes.byref(table), p.data_ptr(), c.data_ptr(), n,
-                                           _lib.dtype_code(p.dtype), ws.data_ptr(), nbytes, _lib.current_stream(dev)),
-                   "fork_sequences")
+        _lib.check(lib.b200_fork_sequences(layers._ref, ctypes.byref(table), p.data_ptr(), c.data_ptr(), n, code,
+                                           ws.data_ptr(), nbytes, _lib.current_stream(dev)), "fork_sequences")
 
 
 def free_sequences(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: torch.Tensor,
@@ -197,16 +199,16 @@ def free_sequences(block_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts
     A page whose count reaches 0 is free.  Naming a row twice, or an empty one, releases
     nothing twice; negative rows are padding.
     """
-    dev = block_table.device
     if ref_counts is None:
         raise ValueError("free_sequences needs ref_counts")
-    table = _table(block_table, seq_lens, ref_counts, max(int(ref_counts.numel()), 1), 1)
-    r = _indices("rows", rows, dev)
-    _cuda(dev, "free_sequences")
+    table, _, dev = _table(block_table, seq_lens, ref_counts, max(ref_counts.numel(), 1), 1)
+    r, n, code = _indices("rows", rows, dev)
+    if dev.type != "cuda":
+        raise RuntimeError("free_sequences runs on CUDA tensors only (no CPU path)")
     lib = _lib.load()
     with _lib.on_device(dev):
-        _lib.check(lib.b200_free_sequences(ctypes.byref(table), r.data_ptr(), r.shape[0], _lib.dtype_code(r.dtype),
-                                           _lib.current_stream(dev)), "free_sequences")
+        _lib.check(lib.b200_free_sequences(ctypes.byref(table), r.data_ptr(), n, code, _lib.current_stream(dev)),
+                   "free_sequences")
 
 
 def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_lens: torch.Tensor,
@@ -223,27 +225,27 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
     that does not rise or has no page of its own, which is recorded.
     """
     layers = cache_layers(kv_caches)
-    dev = layers.device
-    table = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)
-    _same_device(layers, block_table.device)
+    table, rows, dev = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)
     if context_lens.shape != seq_lens.shape or context_lens.dtype != seq_lens.dtype or context_lens.device != dev:
         raise ValueError("context_lens must match seq_lens")
-    if accepted.ndim != 2 or accepted.shape[0] != block_table.shape[0] or accepted.device != dev:
+    if accepted.ndim != 2 or accepted.shape[0] != rows or accepted.device != dev:
         raise ValueError("accepted must have one row per row of the block table")
-    counts = _indices("num_accepted", num_accepted, dev)
-    if counts.shape[0] != accepted.shape[0] or counts.dtype != accepted.dtype:
+    counts, n, code = _indices("num_accepted", num_accepted, dev)
+    if n != rows or counts.dtype != accepted.dtype:
         raise ValueError("num_accepted must hold one count per row, in the dtype of accepted")
-    if abs(context_lens.data_ptr() - seq_lens.data_ptr()) < seq_lens.numel() * seq_lens.element_size():
+    if abs(context_lens.data_ptr() - seq_lens.data_ptr()) < rows * seq_lens.element_size():
         raise ValueError("seq_lens may not be (or overlap) context_lens")
-    _cuda(dev, "keep_accepted_tokens")
-    if accepted.shape[1] and (accepted.stride(1) != 1 or accepted.stride(0) < accepted.shape[1]):
+    _on(layers, dev, "keep_accepted_tokens")
+    most = accepted.shape[1]
+    stride, step = accepted.stride()
+    if most and (step != 1 or stride < most):
         accepted = accepted.contiguous()
+        stride = most
     context_lens = context_lens.contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
         _lib.check(lib.b200_keep_accepted(layers._ref, ctypes.byref(table), context_lens.data_ptr(), accepted.data_ptr(),
-                                          max(accepted.stride(0), accepted.shape[1]), accepted.shape[1],
-                                          counts.data_ptr(), _lib.dtype_code(counts.dtype), _lib.current_stream(dev)),
+                                          max(stride, most), most, counts.data_ptr(), code, _lib.current_stream(dev)),
                    "keep_accepted_tokens")
 
 
