@@ -568,7 +568,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr int kFillsPerTile = kWide ? 4 : 2;  // ring slots per KV tile: K (, K hi), V (, V hi)
   static_assert(!form_rows(kForm) || !kHeadMaps, "plain rows use one map for all heads");
   constexpr bool kStreamed = form_streamed(kForm);
-  griddep_wait();  // launched as a programmatic dependent of the schedule kernel
+  // Launched as a programmatic dependent of the schedule kernel, whose list only the
+  // producer reads: in kFormPrompt it alone waits, and the set-up overlaps the schedule.
+  if (kForm != kFormPrompt) griddep_wait();
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -675,6 +677,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tma_prefetch_desc(&maps.k[lane]);
         tma_prefetch_desc(&maps.v[lane]);
       }
+      if (kForm == kFormPrompt) griddep_wait();
       const int unit_count = kStreamed ? 0 : *a.unit_count;
       int* claim = const_cast<int*>(a.unit_count) + 1;  // reset to 0 by the schedule kernel
       int issued = 0;   // K/V ring fills so far
@@ -1795,6 +1798,10 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
   __syncthreads();
   const int total_units = min(ucarry, a.capacity);
 
+  // A prompt list of at most kSchedThreads units is sorted whole in step 6: its order
+  // before that does not matter, and step 4's passes are skipped.
+  const bool all_tail = kForm != kFormPaged && total_units <= kSchedThreads;
+
   // 4. units per work bucket; each sequence takes a contiguous range of its bucket.
   auto seq_bucket_of = [&](int b, int units) {
     const float keys = fmaxf(static_cast<float>(kv_len(b)) - 0.5f * static_cast<float>(q_len(b)), 1.0f);
@@ -1802,22 +1809,24 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
     return min(kSchedBuckets - 1, max(0, static_cast<int>(__log2f(work) * kSchedBucketsPerOctave)));
   };
   auto seq_units = [&](int b) { return qb[tb[b + 1]] - qb[tb[b]]; };
-  for (int b = threadIdx.x; b < a.num_seqs; b += kSchedThreads) {
-    const int qt = tb[b + 1] - tb[b];
-    if (qt > 0) atomicAdd(&hist[seq_bucket_of(b, qt)], seq_units(b));
-  }
-  __syncthreads();
-  buckets_to_offsets_desc(hist, warp_sums);
-  __syncthreads();
-  for (int b = threadIdx.x; b < a.num_seqs; b += kSchedThreads) {
-    const int qt = tb[b + 1] - tb[b];
-    if (qt > 0) {
-      const int off = atomicAdd(&hist[seq_bucket_of(b, qt)], seq_units(b));
-      a.seq_off[b] = off;
-      if (seq_cached) s_so[b] = off;
+  if (!all_tail) {
+    for (int b = threadIdx.x; b < a.num_seqs; b += kSchedThreads) {
+      const int qt = tb[b + 1] - tb[b];
+      if (qt > 0) atomicAdd(&hist[seq_bucket_of(b, qt)], seq_units(b));
     }
+    __syncthreads();
+    buckets_to_offsets_desc(hist, warp_sums);
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.num_seqs; b += kSchedThreads) {
+      const int qt = tb[b + 1] - tb[b];
+      if (qt > 0) {
+        const int off = atomicAdd(&hist[seq_bucket_of(b, qt)], seq_units(b));
+        a.seq_off[b] = off;
+        if (seq_cached) s_so[b] = off;
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const int* so = seq_cached ? s_so : a.seq_off;
   // 5. scatter, one query unit per thread (adjacent threads write adjacent
   // units): a query unit's units (KV head, then split) go to its sequence's
@@ -1830,7 +1839,7 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
     const int sp = qs[j];
     const int first = qb[j];
     const int qunit = j - tb[seq];
-    const int pos0 = so[seq] + (qb[tb[seq + 1]] - qb[j + 1]);
+    const int pos0 = all_tail ? first : so[seq] + (qb[tb[seq + 1]] - qb[j + 1]);
     const int slot0 = sp > 1 ? qslot[j] * a.num_kv_heads : -1;
     for (int rem = 0; rem < sp * a.num_kv_heads && first + rem < total_units; ++rem) {
       const int kvh = rem / sp;
@@ -1838,7 +1847,7 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
       const int slot = sp > 1 ? slot0 + kvh : -1;
       const int pos = pos0 + rem;
       const int4 u = pack_unit(seq, qunit, kvh, split, sp, slot);
-      if (pos < a.capacity) a.units[pos] = u;
+      if (!all_tail && pos < a.capacity) a.units[pos] = u;
       if (pos >= tail0 && pos < total_units) s_tail[pos - tail0] = u;
       if (sp > 1 && split == 0) a.split_units[slot] = make_int4(seq, qunit, kvh, sp);
     }
@@ -1852,7 +1861,7 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
   int bucket = 0;
   if (mine) {
     // Every tail slot was written in step 5 unless the capacity clipped the list.
-    unit = ucarry == total_units ? s_tail[threadIdx.x] : a.units[tail0 + threadIdx.x];
+    unit = all_tail || ucarry == total_units ? s_tail[threadIdx.x] : a.units[tail0 + threadIdx.x];
     int kvh, split, nsplit;
     unpack_unit(unit, kvh, split, nsplit);
     const int q0 = (seq_cached || kForm != kFormPaged) ? 0 : load_index(a.cu_q, unit.x, a.len_i64);
