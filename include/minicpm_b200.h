@@ -416,7 +416,8 @@ B200_API int b200_prompt_attn_fwd(const B200PromptAttnParams* params, void* stre
  * not seen).  A row that sees no key is 0.  tree_mask: one byte per entry,
  * [total_q, mask_cols], row stride mask_stride.  Everything else as in
  * b200_paged_attn_fwd (the cache layout and its limits) and
- * b200_prompt_attn_fwd (scale, workspace, finiteness).
+ * b200_prompt_attn_fwd (scale, workspace).  Keys and values that some row sees
+ * must be finite; drafted tokens that no row sees may hold anything.
  */
 typedef struct B200TreeAttnParams {
   const void* q;

@@ -1294,7 +1294,39 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
         }  // !fast
         const float neg_m = (m_used == -INFINITY) ? 0.f : -m_used;
-        if (t == last_t && j == n_tiles - 1 && v_tail_from < v_tail_to) {
+        if (kForm == kFormTree) {
+          // V rows that no row of the unit sees may hold anything (NaN included): keys
+          // past the sequence end, drafted tokens that are hidden from all of it.  P is
+          // 0 there but 0 * NaN is NaN, so thread r zeroes row r of the tile if it is one;
+          // the drafted token of the same index is asked first, which mostly sees itself.
+          if ((dual || t == 0) && tile_start + kAttnTileN > ctx) {
+            const int key = tile_start + row, node = key - ctx;
+            bool clear = key >= ug.seq_len && key < slice_up(ug.kv_hi, a.slice);  // slices past that are zero fill
+            if (key < ug.seq_len && node >= 0) {
+              const int npos = min(ppu, ug.q_len - ug.pos0), self = node - ug.pos0;
+              const uint8_t* column = a.tree_mask + static_cast<int64_t>(ug.q_begin + ug.pos0) * a.mask_stride + node;
+              clear = node >= a.mask_cols || self < 0 || self >= npos || column[self * a.mask_stride] == 0;
+              if (clear && node < a.mask_cols)
+                for (int p = 0; p < npos && clear; ++p) clear = column[p * a.mask_stride] == 0;
+            }
+            if (__any_sync(0xffffffffu, clear)) {
+              const int v0 = dual ? (j + 1 == n_tiles ? 2 * n_tiles - 1 : 2 * j + 2) : kFillsPerTile * j + kFillsPerTile / 2;
+              for (int vs = 0; vs < (kWide ? 2 : 1); ++vs) {  // the V slot(s) of the tile
+                const int vidx = unit_fills + v0 + vs;
+                if (!warp_wait(BAR_KV_FULL + vidx % kKvStages, vidx / kKvStages)) {
+                  aborted = true;
+                  break;
+                }
+                const uint32_t vbase = sbase + kSmKV + (vidx % kKvStages) * 32768;
+                if (clear)
+                  for (int i = 0; i < (kNarrow ? 8 : 16); ++i)  // 16-byte pieces
+                    st_shared_v4(vbase + kv_slot_offset<kHeadMaps, kNarrow>(row, i >> 3, i & 7), 0u, 0u, 0u, 0u);
+              }
+              if (aborted) break;
+              fence_proxy_async_smem();
+            }
+          }
+        } else if (t == last_t && j == n_tiles - 1 && v_tail_from < v_tail_to) {
           // Rows of the last page past the sequence end may hold anything (NaN
           // included); P is 0 there but 0 * NaN is NaN, so zero those V rows,
           // as the reference's masked V load does (triton_split_kv_paged.py:122).

@@ -46,8 +46,8 @@ def paged_tree_attention(
     sees drafted token ``j`` of its sequence iff ``tree_mask[t, j]``; it sees every token of
     the context.  A drafted token usually sees itself and its ancestors, but any mask goes;
     a row that sees nothing is 0.  Rows of ``out`` that belong to no sequence are left as
-    they were.  Cached keys and values of a sequence must be finite, those past its length
-    may hold anything.  A lower-triangular mask gives causal attention; one token per
+    they were.  Cached keys and values that some row sees must be finite; drafted tokens that
+    no row sees (slots of a padded draft) and those past a sequence's length may hold anything.  A lower-triangular mask gives causal attention; one token per
     sequence with ``tree_mask[t, 0]`` set is a decode step.
     """
     if q.ndim != 3 or k.ndim != 4 or v.ndim != 4:

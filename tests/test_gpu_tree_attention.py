@@ -151,6 +151,21 @@ def test_masks_that_leave_rows_empty_and_unseen_garbage():
     assert out[4].abs().max().item() == 0.0 and out[29:].abs().max().item() == 0.0
 
 
+@pytest.mark.parametrize("hq,hkv,dim", [(16, 2, 128), (16, 2, 64), (2, 2, 128), (16, 2, 256), (12, 12, 64)])
+@pytest.mark.parametrize("nodes", [5, 20, 100, 150])
+def test_drafted_tokens_that_nobody_sees_may_hold_anything(hq, hkv, dim, nodes):
+    """A padded draft: slots whose K/V rows were never written (NaN) are hidden from every row."""
+    b = Batch([0, 119, 128, 1000], [nodes] * 4, hq=hq, hkv=hkv, dim=dim, seed=nodes)
+    r, mask, cache = random.Random(nodes), b.mask.clone(), b.cache.clone()
+    for row, L in enumerate(b.lens):
+        for j in r.sample(range(nodes), nodes // 3) + [nodes - 1]:
+            mask[row * nodes:(row + 1) * nodes, j] = False
+            pos = L - nodes + j
+            cache[int(b.table[row, pos // b.page]), :, pos % b.page] = float("nan")
+    out = b.run(cache=cache.cuda(), mask=mask)
+    b.check(out, mask=mask)
+
+
 def test_any_mask_goes():
     b = Batch([37, 200], [30, 61], seed=11, width=70)
     mask = torch.rand(b.mask.shape, generator=torch.Generator().manual_seed(1)) < 0.4
