@@ -133,10 +133,10 @@ struct FormLayout {
   bool streamed, shares;  // shares: a unit may be shared by CTAs
   int ctas, ppt, ppu;
   int64_t qunits_ub, capacity;
-  // streamed: CTAs' shared units and partials
-  size_t meta_off, o_off, m_off, l_off;
-  // listed: the schedule kernel's arrays
-  size_t count_off, tile_base_off, seq_off_off, qbase_off, qsplit_off, qslot_off, units_off;
+  // streamed: the CTAs' shared units come first, then their partials
+  size_t o_off, m_off, l_off;
+  // listed: the unit count comes first, then the schedule kernel's arrays
+  size_t tile_base_off, seq_off_off, qbase_off, qsplit_off, qslot_off, units_off;
   size_t total;
 };
 
@@ -259,8 +259,8 @@ int launch_attn_form(const FormLaunch& f, dim3 grid, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto kernel = b200::paged_attn_fwd_kernel<T, kHeadMaps, kWide, kNarrow, kForm>;
   if (int r = prepare_attn_kernel(kernel, done)) return r;
-  return launch_form_kernel("attention kernel", !b200::form_streamed(kForm), kernel, grid, b200::kAttnThreads, b200::kAttnSmemAlloc, s,
-                            f.tm_q, f.maps, f.a);
+  return launch_form_kernel("attention kernel", !b200::form_streamed(kForm), kernel, grid, b200::kAttnThreads,
+                            b200::kAttnSmemAlloc, s, f.tm_q, f.maps, f.a);
 }
 
 template <typename T, bool kHeadMaps, int kForm>
@@ -306,7 +306,7 @@ int launch_schedule(const FormLaunch& f, const FormLayout& w, int sms, cudaStrea
   sa.qunit_split = reinterpret_cast<int*>(ws + w.qsplit_off);
   sa.qunit_slot = reinterpret_cast<int*>(ws + w.qslot_off);
   sa.units = reinterpret_cast<int4*>(ws + w.units_off);
-  sa.unit_count = reinterpret_cast<int*>(ws + w.count_off);
+  sa.unit_count = reinterpret_cast<int*>(ws);
   auto sched = b200::attn_schedule_kernel<kForm>;
   cudaError_t e = cudaFuncSetAttribute(sched, cudaFuncAttributeMaxDynamicSharedMemorySize, b200::kSchedSmemBytes);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "schedule kernel shared memory: %s", cudaGetErrorString(e));
@@ -337,7 +337,7 @@ int run_form(FormLaunch& f, const FormLayout& w, int64_t max_tiles, int sms, cud
     a.l_split = reinterpret_cast<float*>(ws + w.l_off);
   } else {
     a.units = reinterpret_cast<int4*>(ws + w.units_off);
-    a.unit_count = reinterpret_cast<int*>(ws + w.count_off);
+    a.unit_count = reinterpret_cast<int*>(ws);
     if (int r = launch_schedule<kForm>(f, w, sms, s)) return r;
   }
   const dim3 grid((unsigned)w.ctas);

@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           e.k_begin = sb.k_begin;
           if (kForm != kFormPaged) {  // whole units
             e.split = 0;
-            e.nsplit = qunit_full_tiles(e.q_end - e.q_begin, e.seq_len, e.qunit, ppu, kForm == kFormTree ? 1 : a.full);
+            e.nsplit = qunit_full_tiles(e.q_end - e.q_begin, e.seq_len, e.qunit, ppu, a.full);
             e.slot = -1;
           }
         }
@@ -1154,12 +1154,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int unmasked_hi = kForm == kFormTree ? min(ug.split_end, ctx)
                               : full             ? ug.split_end
                                                  : min(ug.split_end, ug.q_abs_min + q_tile * P + 1);
-      // V rows [v_tail_from, v_tail_to) of the last tile: loaded page rows at or past L.
+      // V rows [v_tail_from, v_tail_to) of the last tile: loaded page rows at or past L
+      // (draft trees clear theirs by the mask, below).
       const int last_start = ug.kv_lo + (n_tiles - 1) * kAttnTileN;
       const int v_tail_from = max(ug.seq_len - last_start, 0);
       const int v_tail_to = form_rows(kForm)
                                 ? kAttnTileN
-                                : min(slice_up(ug.kv_hi, kForm == kFormTree ? a.slice : kAttnSlice) - last_start, kAttnTileN);
+                                : min(slice_up(ug.kv_hi, kAttnSlice) - last_start, kAttnTileN);
 
       float m_used = -INFINITY;  // running maximum in scaled base-2 units
       float l = 0.f;
@@ -1731,7 +1732,7 @@ __global__ void __launch_bounds__(kSchedThreads, 1) attn_schedule_kernel(const S
   griddep_launch_dependents();  // the attention grid may launch; it waits for this one
 
   const bool seq_cached = a.num_seqs <= kSchedSeqCache;
-  const int full = kForm == kFormPaged ? 0 : kForm == kFormTree ? 1 : a.full;
+  const int full = kForm == kFormPaged ? 0 : a.full;
   auto q_len = [&](int b) {
     if (seq_cached) return s_ql[b];
     const SeqBounds sb = seq_bounds<kForm>(a, b);

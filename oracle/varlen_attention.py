@@ -1,6 +1,6 @@
 """64-bit CPU restatement of the packed prompt attention and the draft-tree attention.
 
-TEST INFRASTRUCTURE ONLY (the checker; never shipped).  No counterpart in the
+TEST INFRASTRUCTURE ONLY (never shipped).  No counterpart in the
 reference: the operators are defined by their formulas.
 
 Beside the result, :func:`attend` gives what an error bound needs: ``A = sum_j
