@@ -527,7 +527,8 @@ B200_API int b200_free_sequences(const B200SeqTable* table, const void* rows, in
  * released, and a row is not written into a page that is shared.  A path is cut
  * before its first entry that does not rise (B200_DEVERR_ACCEPT), has no page
  * (B200_DEVERR_PAGE_RANGE) or would write a shared page (B200_DEVERR_PAGE_SHARED).
- * seq_lens is written for every row of the table and is not context_lens.
+ * seq_lens is written for every row of the table and overlaps neither context_lens
+ * nor num_accepted.
  */
 B200_API int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable* table, const void* context_lens,
                                 const void* accepted, int64_t accepted_stride, int32_t most, const void* num_accepted,

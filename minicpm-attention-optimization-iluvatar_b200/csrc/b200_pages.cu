@@ -204,7 +204,8 @@ int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable* table, 
   if (!index_type(index_dtype)) return fail(B200_ERR_INVALID, "accepted and num_accepted must be int32 or int64");
   if (most < 0 || accepted_stride < most) return fail(B200_ERR_INVALID, "bad sizes");
   if (a.t.max_seqs == 0) return B200_OK;
-  if (context_lens == a.t.seq_lens) return fail(B200_ERR_INVALID, "seq_lens may not be context_lens");
+  if (context_lens == a.t.seq_lens || num_accepted == a.t.seq_lens)
+    return fail(B200_ERR_INVALID, "seq_lens may not be context_lens or num_accepted");
   if (!context_lens || !num_accepted || (most > 0 && !accepted)) return fail(B200_ERR_INVALID, "null lengths or path");
   a.s = c.shape;
   a.context_lens = context_lens;

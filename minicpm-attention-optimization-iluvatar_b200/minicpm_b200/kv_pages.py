@@ -235,6 +235,9 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
         raise ValueError("num_accepted must hold one count per row, in the dtype of accepted")
     if abs(context_lens.data_ptr() - seq_lens.data_ptr()) < rows * seq_lens.element_size():
         raise ValueError("seq_lens may not be (or overlap) context_lens")
+    lens_end = seq_lens.data_ptr() + rows * seq_lens.element_size()  # other sequences' counts are read while it is written
+    if counts.data_ptr() < lens_end and seq_lens.data_ptr() < counts.data_ptr() + rows * counts.element_size():
+        raise ValueError("seq_lens may not be (or overlap) num_accepted")
     _on(layers, dev, "keep_accepted_tokens")
     most = accepted.shape[1]
     stride, step = accepted.stride()

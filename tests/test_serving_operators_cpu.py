@@ -184,6 +184,22 @@ def test_copy_free_and_keep_refusals():
         keep()
 
 
+@pytest.mark.parametrize("lens_type", [torch.int32, torch.int64])
+def test_keep_refuses_counts_that_its_lengths_overwrite(lens_type):
+    # Several warps read a sequence's count; the first to finish stores its length.
+    p = _pool(seq_lens=torch.zeros(3, dtype=lens_type))
+    ctx, acc = torch.zeros(3, dtype=lens_type), torch.zeros(3, 2, dtype=torch.int32)
+    shared = torch.zeros(12, dtype=torch.int32)
+    for counts, at in [(shared[:3], 0), (shared[1:4], 0), (shared[2:5], 0)]:
+        lens = shared.view(lens_type).as_strided((3,), (1,), at)
+        with pytest.raises(ValueError, match="num_accepted"):
+            kv_pages.keep_accepted_tokens(p["kv_caches"], p["block_table"], ctx, acc, counts, lens)
+    lens = shared.view(lens_type)[:3]
+    apart = shared[lens.element_size() // 4 * 3:][:3]
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):  # behind them: accepted, up to the device
+        kv_pages.keep_accepted_tokens(p["kv_caches"], p["block_table"], ctx, acc, apart, lens)
+
+
 def test_c_entries_return_a_status():
     lib = _lib.load()
     assert lib.b200_prompt_attn_fwd(None, None) == _lib.B200_ERR_INVALID
