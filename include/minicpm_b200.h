@@ -502,7 +502,9 @@ B200_API int b200_copy_pages(const B200PageCaches* caches, const void* src_pages
  * (length 0) and is named once.  Entries with a negative index are padding.  An
  * entry that cannot be served (a row out of range, in use or named before:
  * B200_DEVERR_SEQ_ROW; no page left: B200_DEVERR_NO_PAGE; a table that names no
- * page: B200_DEVERR_PAGE_RANGE) is recorded and leaves its child empty.
+ * page for the partial last one: B200_DEVERR_PAGE_RANGE) is recorded and leaves its
+ * child empty.  A full page that the parent's row does not name is missing in the
+ * child's row too (-1), and is recorded the same way.
  * workspace: b200_fork_workspace_bytes(num_entries, max_seqs), 16-byte aligned.
  */
 B200_API size_t b200_fork_workspace_bytes(int32_t num_entries, int32_t max_seqs);
@@ -527,6 +529,8 @@ B200_API int b200_free_sequences(const B200SeqTable* table, const void* rows, in
  * released, and a row is not written into a page that is shared.  A path is cut
  * before its first entry that does not rise (B200_DEVERR_ACCEPT), has no page
  * (B200_DEVERR_PAGE_RANGE) or would write a shared page (B200_DEVERR_PAGE_SHARED).
+ * A context that is no length (negative, past 2^30 - 1) is recorded as
+ * B200_DEVERR_ACCEPT: the row's length becomes 0 and it keeps its pages.
  * seq_lens is written for every row of the table and overlaps neither context_lens
  * nor num_accepted.
  */

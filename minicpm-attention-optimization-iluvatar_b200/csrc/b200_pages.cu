@@ -226,6 +226,7 @@ int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable* table, 
   b200::FreeArgs fa{};
   fa.t = a.t;
   fa.n = a.num_seqs;
+  fa.context_lens = context_lens;
   return launch_after("free_pages_kernel", b200::free_pages_kernel<0>, dim3((unsigned)a.num_seqs), s, fa);
 }
 

@@ -39,6 +39,8 @@ __device__ __forceinline__ void store_index(void* p, int64_t i, int is_i64, int 
   if (is_i64) static_cast<int64_t*>(p)[i] = v;
   else static_cast<int*>(p)[i] = v;
 }
+// A length that token positions held in 32 bits can start from.
+__device__ __forceinline__ bool is_context(int64_t len) { return len >= 0 && len <= 0x3fffffff; }
 // Takes the entry out of the table: -1 stays, the caller that gets the page owns its release.
 __device__ __forceinline__ int64_t take_index(void* p, int64_t i, int is_i64) {
   if (is_i64) return static_cast<int64_t>(atomicExch(static_cast<unsigned long long*>(p) + i, ~0ull));
@@ -148,7 +150,8 @@ __global__ void __launch_bounds__(kForkThreads, 1) fork_plan_kernel(const ForkAr
     if (i < a.n && entry(i, p, c)) {
       const int64_t len64 = load_index64(a.t.seq_lens, p, a.t.len_i64);
       ok = true;
-      if (*reinterpret_cast<volatile int*>(&a.claims[c]) != i || load_index64(a.t.seq_lens, c, a.t.len_i64) != 0 || len64 < 0 ||
+      const bool claimed = *reinterpret_cast<volatile int*>(&a.claims[c]) == i;
+      if (!claimed || load_index64(a.t.seq_lens, c, a.t.len_i64) != 0 || !is_context(len64) ||
           len64 > static_cast<int64_t>(a.t.cols) * a.t.block_size) {
         record_device_error(B200_DEVERR_SEQ_ROW);  // a row named twice, one in use, a length past the table
         ok = false;
@@ -272,6 +275,7 @@ __global__ void __launch_bounds__(kPageThreads) fork_apply_kernel(const __grid_c
 struct FreeArgs {
   SeqTable t;
   const void* rows;   // [n] rows to empty, or null: rows 0 .. n - 1 keep the pages that their length needs
+  const void* context_lens;  // rows null: a row whose context is no length keeps all its pages
   int n, idx_i64;
 };
 
@@ -288,6 +292,7 @@ __global__ void __launch_bounds__(kPageThreads) free_pages_kernel(const FreeArgs
   }
   int64_t first = 0;
   if (!a.rows) {
+    if (!is_context(load_index64(a.context_lens, row, a.t.len_i64))) return;  // the keep kernel has recorded it
     const int64_t len = max(load_index64(a.t.seq_lens, row, a.t.len_i64), static_cast<int64_t>(0));
     first = (len + a.t.block_size - 1) / a.t.block_size;
   }
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(kPageThreads) keep_accepted_kernel(const __gri
     const bool first_unit = blockIdx.y == 0 && x == lane;  // reports errors and stores the length
     const int64_t ctx64 = load_index64(a.context_lens, b, a.t.len_i64);
     const int64_t want = load_index64(a.counts, b, a.idx_i64);
-    const bool bad_ctx = ctx64 < 0 || ctx64 > 0x3fffffff, bad = bad_ctx || want < 0 || want > a.most;
+    const bool bad_ctx = !is_context(ctx64), bad = bad_ctx || want < 0 || want > a.most;
     const int ctx = bad_ctx ? 0 : static_cast<int>(ctx64);
     int n = bad_ctx || want < 0 ? 0 : static_cast<int>(min(want, static_cast<int64_t>(a.most)));
     const int64_t trow = static_cast<int64_t>(b) * a.t.stride, arow = static_cast<int64_t>(b) * a.acc_stride;

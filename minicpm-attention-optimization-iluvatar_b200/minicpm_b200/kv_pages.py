@@ -171,7 +171,8 @@ def fork_sequences(kv_caches: Caches, block_table: torch.Tensor, seq_lens: torch
     copied, in every layer, to a page of the child's own: the lowest free pages, given out in
     the order of the entries.  The child's row must be empty (length 0) and is named once; a
     parent may have any number of children.  Entries with a negative index are padding; one
-    that cannot be served leaves its child empty and is recorded.
+    that cannot be served leaves its child empty and is recorded.  A full page that the
+    parent's row does not name is missing in the child's row too (-1), and is recorded.
     """
     layers = cache_layers(kv_caches)
     table, rows, dev = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)
@@ -222,7 +223,8 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
     among the drafted tokens, strictly rising; what is behind ``num_accepted[b]`` is not read.
     With ``ref_counts`` the pages behind the new lengths are released (their table entries
     become -1) and a shared page is not written to.  A path is cut before its first entry
-    that does not rise or has no page of its own, which is recorded.
+    that does not rise or has no page of its own, which is recorded; a negative context is
+    recorded too, its row keeps its pages and gets length 0.
     """
     layers = cache_layers(kv_caches)
     table, rows, dev = _table(block_table, seq_lens, ref_counts, layers.num_blocks, layers.block_size)

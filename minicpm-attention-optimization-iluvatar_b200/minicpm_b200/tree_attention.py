@@ -47,8 +47,9 @@ def paged_tree_attention(
     the context.  A drafted token usually sees itself and its ancestors, but any mask goes;
     a row that sees nothing is 0.  Rows of ``out`` that belong to no sequence are left as
     they were.  Cached keys and values that some row sees must be finite; drafted tokens that
-    no row sees (slots of a padded draft) and those past a sequence's length may hold anything.  A lower-triangular mask gives causal attention; one token per
-    sequence with ``tree_mask[t, 0]`` set is a decode step.
+    no row sees (slots of a padded draft) and those past a sequence's length may hold
+    anything.  A lower-triangular mask gives causal attention; one token per sequence with
+    ``tree_mask[t, 0]`` set is a decode step.
     """
     if q.ndim != 3 or k.ndim != 4 or v.ndim != 4:
         raise ValueError("expected q=[T,H,D] and k/v=[blocks,block,kv_heads,D]")

@@ -276,6 +276,38 @@ def test_keep_refuses_bad_paths():
     assert _lib.device_error() in (_lib.DEVERR_ACCEPT, _lib.DEVERR_PAGE_RANGE)
 
 
+@pytest.mark.parametrize("index,bad", [(torch.int32, -1), (torch.int64, -(1 << 40)), (torch.int64, 1 << 40)])
+def test_keep_leaves_the_pages_of_a_bad_context(index, bad):
+    page = 16
+    caches = _caches(1, 12, page, 1, 64, torch.bfloat16, seed=3)
+    pool = Pool([40, 50], 0, page, 12, 4, caches, index)
+    gpu, layers = _layers(caches)
+    table, lens, refs = pool.gpu()
+    ctx = torch.tensor([bad, 30], dtype=index).cuda()
+    acc, num = torch.tensor([[0, 1], [0, 1]], dtype=index).cuda(), torch.tensor([2, 2], dtype=index).cuda()
+    kv_pages.keep_accepted_tokens(layers, table, ctx, acc, num, lens, refs)
+    pool.lens = [0, 32]  # row 0 still names its pages; row 1 gives back the two behind 32 tokens
+    for col in (2, 3):
+        pool.refs[pool.table[1][col]] -= 1
+        pool.table[1][col] = -1
+    pool.check(table, lens, refs, gpu)
+    assert _lib.device_error() == _lib.DEVERR_ACCEPT
+    kv_pages.free_sequences(table, lens, refs, torch.tensor([0]).cuda())
+    assert (table[0] == -1).all() and refs.sum().item() == 2
+
+
+def test_fork_of_a_parent_that_lacks_a_full_page():
+    caches = _caches(1, 8, 16, 1, 64, torch.bfloat16)
+    pool = Pool([40], 2, 16, 8, 4, caches)
+    _, layers = _layers(caches)
+    table, lens, refs = pool.gpu()
+    table[0, 0] = -1
+    kv_pages.fork_sequences(layers, table, lens, refs, torch.tensor([0]).cuda(), torch.tensor([1]).cuda())
+    row = table[1].tolist()
+    assert row[0] == -1 and row[1] == int(table[0, 1]) and row[2] >= 0 and row[3] == -1
+    assert refs[row[1]].item() == 2 and refs[row[2]].item() == 1 and _lib.device_error() == _lib.DEVERR_PAGE_RANGE
+
+
 def test_keep_does_not_write_shared_pages():
     page = 16
     caches = _caches(1, 12, page, 1, 64, torch.bfloat16, seed=3)
