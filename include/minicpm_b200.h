@@ -498,12 +498,13 @@ B200_API int b200_copy_pages(const B200PageCaches* caches, const void* src_pages
  * Row children[i] of the table becomes a copy of row parents[i]: full pages are
  * shared (their counts rise by one), the used rows of a partial last page go to a
  * free page of the child's own -- the lowest free ones, in the order of the
- * entries -- and seq_lens[child] = seq_lens[parent].  A child's row must be empty
- * (length 0) and is named once.  Entries with a negative index are padding.  An
- * entry that cannot be served (a row out of range, in use or named before:
+ * entries -- and seq_lens[child] = seq_lens[parent].  A child's row must have
+ * length 0 and is named once; pages that it names all the same (reserved ones) are
+ * released, and are not given out by the same call.  Entries with a negative index
+ * are padding.  An entry that cannot be served (a row out of range, in use or named before:
  * B200_DEVERR_SEQ_ROW; no page left: B200_DEVERR_NO_PAGE; a table that names no
  * page for the partial last one: B200_DEVERR_PAGE_RANGE) is recorded and leaves its
- * child empty.  A full page that the parent's row does not name is missing in the
+ * child as it was.  A full page that the parent's row does not name is missing in the
  * child's row too (-1), and is recorded the same way.
  * workspace: b200_fork_workspace_bytes(num_entries, max_seqs), 16-byte aligned.
  */

@@ -46,6 +46,15 @@ __device__ __forceinline__ int64_t take_index(void* p, int64_t i, int is_i64) {
   if (is_i64) return static_cast<int64_t>(atomicExch(static_cast<unsigned long long*>(p) + i, ~0ull));
   return atomicExch(static_cast<int*>(p) + i, -1);
 }
+// One row of the table no longer names `page` (not negative): its count goes down.
+__device__ __forceinline__ void release_page(int* ref_counts, int64_t page, int num_blocks) {
+  if (page >= num_blocks) {
+    record_device_error(B200_DEVERR_PAGE_RANGE);
+  } else if (atomicSub(&ref_counts[page], 1) <= 0) {
+    atomicAdd(&ref_counts[page], 1);  // was free already
+    record_device_error(B200_DEVERR_PAGE_RANGE);
+  }
+}
 
 // V: 16 bytes, or 4 for the caches whose rows carry a float32 scale inline.
 template <typename V>
@@ -229,6 +238,11 @@ __global__ void __launch_bounds__(kPageThreads) fork_apply_kernel(const __grid_c
       const int4 e = a.entries[i];
       if (e.y < 0 || col >= a.t.cols) continue;
       const int full = e.z / a.t.block_size;
+      // A row of length 0 may name pages all the same (reserved ones, those of a context
+      // that was no length): they go back.  The plan was made by the counts before, so none
+      // of them is given out by this call.
+      const int64_t old = load_index64(a.t.table, e.y * a.t.stride + col, a.t.table_i64);
+      if (old >= 0) release_page(a.t.ref_counts, old, a.t.num_blocks);
       int64_t page = -1;
       if (col < full) {
         page = load_index64(a.t.table, e.x * a.t.stride + col, a.t.table_i64);
@@ -299,13 +313,7 @@ __global__ void __launch_bounds__(kPageThreads) free_pages_kernel(const FreeArgs
   for (int64_t col = first + threadIdx.x; col < a.t.cols; col += kPageThreads) {
     if (load_index64(a.t.table, row * a.t.stride + col, a.t.table_i64) < 0) continue;
     const int64_t page = take_index(a.t.table, row * a.t.stride + col, a.t.table_i64);
-    if (page < 0) continue;
-    if (page >= a.t.num_blocks) {
-      record_device_error(B200_DEVERR_PAGE_RANGE);
-    } else if (atomicSub(&a.t.ref_counts[page], 1) <= 0) {
-      atomicAdd(&a.t.ref_counts[page], 1);  // was free already
-      record_device_error(B200_DEVERR_PAGE_RANGE);
-    }
+    if (page >= 0) release_page(a.t.ref_counts, page, a.t.num_blocks);
   }
   if (a.rows && threadIdx.x == 0) store_index(a.t.seq_lens, row, a.t.len_i64, 0);
 }

@@ -169,9 +169,10 @@ def fork_sequences(kv_caches: Caches, block_table: torch.Tensor, seq_lens: torch
 
     Full pages are shared and their counts rise; the used rows of a partial last page are
     copied, in every layer, to a page of the child's own: the lowest free pages, given out in
-    the order of the entries.  The child's row must be empty (length 0) and is named once; a
+    the order of the entries.  The child's row must have length 0 and is named once; pages that
+    it names all the same (reserved ones) are released, and are not given out by the same call.  A
     parent may have any number of children.  Entries with a negative index are padding; one
-    that cannot be served leaves its child empty and is recorded.  A full page that the
+    that cannot be served leaves its child as it was and is recorded.  A full page that the
     parent's row does not name is missing in the child's row too (-1), and is recorded.
     """
     layers = cache_layers(kv_caches)
