@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(kCombineThreads) stream_combine_kernel(const S
   const int cta = blockIdx.x;
   const int4 su = a.meta[cta];
   if (su.w == 0) return;
-  const int q_begin = min(max(load_index(a.cu_q, su.x, a.len_i64), 0), a.total_q);
-  const int q_end = min(load_index(a.cu_q, su.x + 1, a.len_i64), a.total_q);
+  const int q_begin = load_clipped(a.cu_q, su.x, a.len_i64, 0, a.total_q);  // the rows that the pieces hold (seq_bounds)
+  const int q_end = load_clipped(a.cu_q, su.x + 1, a.len_i64, q_begin, a.total_q);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto place = [&](int ur, int64_t& tok, int64_t& head) -> bool {  // where row ur of the unit goes, if it exists
     const int t = ur / kAttnTileM, r = ur % kAttnTileM;
