@@ -418,6 +418,9 @@ B200_API int b200_prompt_attn_fwd(const B200PromptAttnParams* params, void* stre
  * b200_paged_attn_fwd (the cache layout and its limits) and
  * b200_prompt_attn_fwd (scale, workspace).  Keys and values that some row sees
  * must be finite; drafted tokens that no row sees may hold anything.
+ * The batch's units of work (query tile pairs x KV heads, one per sequence and KV
+ * head at least) times the KV tiles of a full table row stay below 2^30, or the
+ * call is refused: 256 sequences of 8 KV heads with tables of 2^24 keys each pass.
  */
 typedef struct B200TreeAttnParams {
   const void* q;

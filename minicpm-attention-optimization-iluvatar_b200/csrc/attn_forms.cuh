@@ -202,6 +202,25 @@ inline FormLayout form_layout(bool streamed, int64_t total_q, int num_seqs, int 
   return w;
 }
 
+// Streamed shares count ticks in 32 bits: no batch of these sizes may reach 2^31 of
+// them, even if one sequence has every key (max_tiles KV tiles).  Prompts that could
+// take the list, which counts units.
+inline bool ticks_fit(const FormLayout& w, int64_t max_tiles) {
+  return w.capacity <= 0x7fffffff / (b200::kStreamOverhead + 2 * max_tiles);
+}
+
+// The limits of a layout, before anything is done on the GPU.
+inline int check_layout(const FormLayout& w, int64_t max_tiles, const void* workspace, size_t workspace_bytes) {
+  if (w.capacity > 0x7fffffff) return fail(B200_ERR_UNSUPPORTED, "more than 2^31 units of work in one call");
+  if (w.streamed && !ticks_fit(w, max_tiles))
+    return fail(B200_ERR_UNSUPPORTED, "units of work (%lld) times their KV tiles (up to %lld) pass 2^30 in one call",
+                (long long)w.capacity, (long long)max_tiles);
+  if (!workspace || workspace_bytes < w.total)
+    return fail(B200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", w.total, workspace_bytes);
+  if (!aligned16(workspace)) return fail(B200_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  return B200_OK;
+}
+
 // What a form's entry point hands over: maps and kernel arguments that only it
 // knows, the rest is filled in here.
 struct FormLaunch {
@@ -209,9 +228,8 @@ struct FormLaunch {
   b200::KvHeadMaps maps;
   b200::AttnKernelArgs a;
   bool head_maps;
-  int dtype, num_seqs, num_kv_heads, max_seqlen_k;
-  void* workspace;
-  size_t workspace_bytes;
+  int dtype, num_seqs, num_kv_heads;
+  void* workspace;  // checked (check_layout)
 };
 
 // Once per kernel and device: the register count that the kernel's setmaxnreg
@@ -314,15 +332,10 @@ int launch_schedule(const FormLaunch& f, const FormLayout& w, int sms, cudaStrea
   return check_launch("attn_schedule_kernel");
 }
 
-// `w` lies in the workspace; max_tiles bounds the KV tiles of a sequence by the caller's sizes.
+// `w` lies in the workspace.
 template <int kForm>
-int run_form(FormLaunch& f, const FormLayout& w, int64_t max_tiles, int sms, cudaStream_t s) {
+int run_form(FormLaunch& f, const FormLayout& w, int sms, cudaStream_t s) {
   b200::AttnKernelArgs& a = f.a;
-  if (w.capacity * (b200::kStreamOverhead + 2 * max_tiles) > 0x7fffffff)
-    return fail(B200_ERR_UNSUPPORTED, "more than 2^30 KV tiles of work in one call");
-  if (!f.workspace || f.workspace_bytes < w.total)
-    return fail(B200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", w.total, f.workspace_bytes);
-  if (!aligned16(f.workspace)) return fail(B200_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(f.workspace);
   a.pos_per_tile = w.ppt;
   a.num_seqs = f.num_seqs;

@@ -39,8 +39,19 @@ int b200_prompt_attn_fwd(const B200PromptAttnParams* p, void* stream) {
   if (((p->k_stride_t | p->k_stride_h | p->v_stride_t | p->v_stride_h) * 2) & 15)
     return fail(B200_ERR_UNSUPPORTED, "token/head strides must be multiples of 16 bytes");
 
-  FormLaunch f{};
   const int group = p->num_q_heads / p->num_kv_heads, ppt = b200::kAttnTileM / group;
+  const int sms = sm_count();
+  const int ppu = ppt * (p->head_dim == 256 ? 1 : b200::kAttnTilesPerUnit);
+  const int64_t max_tiles = (int64_t)p->total_k / b200::kAttnTileN + 1;
+  auto layout = [&](bool streamed) {
+    return form_layout(streamed, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim, p->max_seqlen_k, sms);
+  };
+  FormLayout w = layout(stream_prompt(p->total_q, p->total_k, p->num_seqs, ppu, p->num_kv_heads, p->max_seqlen_k,
+                                      p->causal != 0, sms));
+  if (w.streamed && !ticks_fit(w, max_tiles)) w = layout(false);
+  if (int r = check_layout(w, max_tiles, p->workspace, p->workspace_bytes)) return r;
+
+  FormLaunch f{};
   if (int r = encode_rows(&f.tm_q, p->dtype, p->q, p->head_dim, p->num_q_heads, p->total_q, p->q_stride_t,
                           p->q_stride_h, group, ppt, "q"))
     return r;
@@ -57,9 +68,7 @@ int b200_prompt_attn_fwd(const B200PromptAttnParams* p, void* stream) {
   f.dtype = p->dtype;
   f.num_seqs = p->num_seqs;
   f.num_kv_heads = p->num_kv_heads;
-  f.max_seqlen_k = p->max_seqlen_k;
   f.workspace = p->workspace;
-  f.workspace_bytes = p->workspace_bytes;
   b200::AttnKernelArgs& a = f.a;
   a.cu_q = p->cu_seqlens_q;
   a.cu_k = p->cu_seqlens_k;
@@ -75,16 +84,8 @@ int b200_prompt_attn_fwd(const B200PromptAttnParams* p, void* stream) {
   a.block_size = 1;
   a.full = p->causal ? 0 : 1;
   a.scale_log2 = static_cast<float>(static_cast<double>(p->softmax_scale) * 1.4426950408889634);
-  const int sms = sm_count();
-  const int ppu = ppt * (p->head_dim == 256 ? 1 : b200::kAttnTilesPerUnit);
-  const bool streamed = stream_prompt(p->total_q, p->total_k, p->num_seqs, ppu, p->num_kv_heads, p->max_seqlen_k,
-                                      p->causal != 0, sms);
-  const FormLayout w = form_layout(streamed, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim,
-                                   p->max_seqlen_k, sms);
-  const int64_t max_tiles = (int64_t)p->total_k / b200::kAttnTileN + 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return w.streamed ? run_form<b200::kFormPromptStream>(f, w, max_tiles, sms, s)
-                    : run_form<b200::kFormPrompt>(f, w, max_tiles, sms, s);
+  return w.streamed ? run_form<b200::kFormPromptStream>(f, w, sms, s) : run_form<b200::kFormPrompt>(f, w, sms, s);
 }
 
 }  // extern "C"

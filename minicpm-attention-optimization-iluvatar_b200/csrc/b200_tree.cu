@@ -69,6 +69,12 @@ int b200_tree_attn_fwd(const B200TreeAttnParams* p, void* stream) {
         p->v_stride_head) * 2) & 15)
     return fail(B200_ERR_UNSUPPORTED, "token/head/block strides must be multiples of 16 bytes");
 
+  const int sms = sm_count();
+  const FormLayout w = form_layout(true, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim,
+                                   p->max_seqlen_k, sms);
+  const int64_t max_tiles = (int64_t)p->block_table_cols * p->block_size / b200::kAttnTileN + 1;
+  if (int r = check_layout(w, max_tiles, p->workspace, p->workspace_bytes)) return r;
+
   FormLaunch f{};
   const int group = p->num_q_heads / p->num_kv_heads, ppt = b200::kAttnTileM / group;
   if (int r = encode_rows(&f.tm_q, p->dtype, p->q, p->head_dim, p->num_q_heads, p->total_q, p->q_stride_t,
@@ -83,9 +89,7 @@ int b200_tree_attn_fwd(const B200TreeAttnParams* p, void* stream) {
   f.dtype = p->dtype;
   f.num_seqs = p->num_seqs;
   f.num_kv_heads = p->num_kv_heads;
-  f.max_seqlen_k = p->max_seqlen_k;
   f.workspace = p->workspace;
-  f.workspace_bytes = p->workspace_bytes;
   b200::AttnKernelArgs& a = f.a;
   a.block_table = p->block_table;
   a.cu_q = p->cu_seqlens_q;
@@ -109,11 +113,7 @@ int b200_tree_attn_fwd(const B200TreeAttnParams* p, void* stream) {
   a.mask_cols = p->mask_cols;
   a.full = 1;
   a.scale_log2 = static_cast<float>(static_cast<double>(p->softmax_scale) * 1.4426950408889634);
-  const int sms = sm_count();
-  const FormLayout w = form_layout(true, p->total_q, p->num_seqs, p->num_q_heads, p->num_kv_heads, p->head_dim,
-                                   p->max_seqlen_k, sms);
-  const int64_t max_tiles = (int64_t)p->block_table_cols * p->block_size / b200::kAttnTileN + 1;
-  return run_form<b200::kFormTree>(f, w, max_tiles, sms, static_cast<cudaStream_t>(stream));
+  return run_form<b200::kFormTree>(f, w, sms, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

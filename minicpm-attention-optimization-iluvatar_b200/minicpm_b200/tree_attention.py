@@ -50,6 +50,9 @@ def paged_tree_attention(
     no row sees (slots of a padded draft) and those past a sequence's length may hold
     anything.  A lower-triangular mask gives causal attention; one token per sequence with
     ``tree_mask[t, 0]`` set is a decode step.
+
+    The batch's units of work (one per sequence and KV head at least) times the 128-key tiles
+    of a full row of the block table stay below 2^30, else ``RuntimeError``.
     """
     if q.ndim != 3 or k.ndim != 4 or v.ndim != 4:
         raise ValueError("expected q=[T,H,D] and k/v=[blocks,block,kv_heads,D]")
