@@ -22,6 +22,23 @@ from . import _lib
 
 _INDEX_TYPES = (torch.int32, torch.int64)
 _ELEMENT_TYPES = (torch.bfloat16, torch.float16)
+_MAX_SCALE = 3.0e38
+
+
+def prompt_layout_supported(*rows: torch.Tensor, softmax_scale: float) -> bool:
+    """Whether the kernel can address these ``[T, H, D]`` tensors, and takes the scale.
+
+    For callers that have another kernel for such a call; types and head shapes are
+    :func:`~minicpm_b200.split_kv_paged.kernel_supports`'s part.
+    """
+    for t in rows:
+        if t.ndim != 3:
+            return False
+        tokens, heads, _ = t.shape
+        st, sh, sd = t.stride()
+        if sd != 1 or t.data_ptr() % 16 or (heads > 1 and sh % 8) or (tokens > 1 and st % 8):
+            return False
+    return 0.0 < softmax_scale <= _MAX_SCALE
 
 
 def prompt_attention(
@@ -77,7 +94,7 @@ def prompt_attention(
         raise ValueError("k and v hold fewer rows than q: pass cu_seqlens_k")
     if max_seqlen_k is None:
         max_seqlen_k = max_seqlen_q if same_k else total_k
-    if not 0.0 < softmax_scale <= 3.0e38:
+    if not 0.0 < softmax_scale <= _MAX_SCALE:
         raise ValueError("softmax_scale must be positive and finite")
     if not q.is_cuda:
         raise RuntimeError("prompt_attention runs on CUDA tensors only (no CPU path)")

@@ -20,7 +20,8 @@ reference's integration patch adds it (``integration/vllm-plugin-FL-split-kv.pat
   ``do_kv_cache_update`` (the sm_100a cache writers of :mod:`.kv_cache`) and
   ``do_rope_and_kv_cache_update`` (the fused RoPE + cache write).
   Encoder batches run :func:`~minicpm_b200.prompt_attention` when both flags are
-  set and the call has no sliding window, bias or unsupported shape, else vLLM's
+  set and the call has no sliding window or bias and a shape, rows (16-byte aligned,
+  strides of whole 8 elements) and a scale that the kernel takes, else vLLM's
   ``context_attention_fwd`` as in the reference.
 * :class:`IluvatarAttentionMetadata`, :class:`IluvatarAttentionMetadataBuilder`
   and :class:`IluvatarAttentionBackend` (patch :150-466) -- the metadata, its
@@ -72,7 +73,7 @@ from .kv_cache import (
     reshape_and_cache_flash_per_token_head_quant,
     rope_and_cache,
 )
-from .prompt_attention import prompt_attention
+from .prompt_attention import prompt_attention, prompt_layout_supported
 from .split_kv_paged import kernel_supports
 from .unified_attention_optimized import unified_attention_optimized
 
@@ -514,12 +515,13 @@ class IluvatarAttentionImpl:
 
     def _forward_encoder_attention(self, query, key, value, output, attn_metadata, layer) -> torch.Tensor:
         """Bidirectional attention without a cache: ``prompt_attention`` (both flags set, no window or
-        bias, a shape the kernel runs), else vLLM's ``context_attention_fwd`` as in the reference."""
+        bias, a shape and rows that the kernel takes), else vLLM's ``context_attention_fwd`` as in the reference."""
         if is_quantized_kv_cache(self.kv_cache_dtype):
             raise NotImplementedError("quantized KV cache is not supported for encoder attention")
         if (_flag("ILUVATAR_USE_OPTIMIZED") and _flag("ILUVATAR_SPLIT_KV") and self.sliding_window == (-1, -1)
                 and self.alibi_slopes is None and self.sinks is None and not self.logits_soft_cap
-                and kernel_supports(query, key.unsqueeze(0)) and value.dtype == query.dtype == output.dtype):
+                and kernel_supports(query, key.unsqueeze(0)) and value.dtype == query.dtype == output.dtype
+                and prompt_layout_supported(query, key, value, output, softmax_scale=self.scale)):
             return prompt_attention(query, key, value, output, attn_metadata.query_start_loc, attn_metadata.max_query_len,
                                     self.scale, causal=False)
         try:
