@@ -477,6 +477,7 @@ class IluvatarAttentionImpl:
             v_descale = layer._v_scale.expand(descale_shape) if quantized else None
             k_scale_cache = v_scale_cache = None
 
+        tree_mask = getattr(attn_metadata, "tree_mask", None)  # metadata of other makers has no such field
         _run_unified_attention(
             q=query[:n],
             k=key_cache,
@@ -509,7 +510,7 @@ class IluvatarAttentionImpl:
             v_scale_cache=v_scale_cache,
             chunk_lookback=self.chunk_lookback,
             use_td=self.use_td,
-            **({} if attn_metadata.tree_mask is None else {"tree_mask": attn_metadata.tree_mask[:n]}),
+            **({} if tree_mask is None else {"tree_mask": tree_mask[:n]}),
         )
         return output
 
