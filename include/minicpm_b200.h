@@ -372,7 +372,7 @@ B200_API size_t b200_varlen_attn_workspace_bytes(int32_t total_q, int32_t num_se
  * q, out [total_q, num_q_heads, head_dim]; k, v [total_k, num_kv_heads, head_dim];
  * d contiguous, other strides multiples of 8 elements, pointers 16-byte aligned.
  * F16 / BF16, head_dim 64, 128 or 256, up to 128 query heads per KV head.
- * softmax_scale must be positive and finite.  max_seqlen_k bounds the longest
+ * softmax_scale must be positive and at most 2e38.  max_seqlen_k bounds the longest
  * sequence and only decides how far the keys may be split.
  * Keys and values that some row of the tile sees must be finite; rows of k and v
  * outside every sequence may hold anything.

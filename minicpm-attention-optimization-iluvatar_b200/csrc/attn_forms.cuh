@@ -403,8 +403,9 @@ inline int check_form(const FormShape& p) {
   if (p.seqlen_dtype != B200_DTYPE_I32 && p.seqlen_dtype != B200_DTYPE_I64)
     return fail(B200_ERR_INVALID, "sequence lengths must be int32 or int64");
   if (p.num_seqs < 0 || p.total_q < 0) return fail(B200_ERR_INVALID, "bad sizes");
-  // The running maximum is taken over unscaled scores, so the scale keeps their order.
-  if (!(p.scale > 0.f) || p.scale > 3.0e38f) return fail(B200_ERR_INVALID, "softmax_scale must be positive and finite");
+  // The running maximum is taken over unscaled scores, so the scale keeps their order;
+  // times log2(e) it is finite (2.36e38 would not be), or scores of 0 would give NaN.
+  if (!(p.scale > 0.f) || p.scale > 2.0e38f) return fail(B200_ERR_INVALID, "softmax_scale must be positive and at most 2e38");
   if (p.total_q == 0 || p.num_seqs == 0) return B200_OK;
   if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.out))
     return fail(B200_ERR_UNSUPPORTED, "q, k, v and out must be 16-byte aligned");

@@ -52,6 +52,9 @@ DEVERR_PAGE_RANGE = 7
 DEVERR_PAGE_SHARED = 8
 DEVERR_ACCEPT = 9
 
+# Largest softmax_scale of the prompt and tree kernels: times log2(e) it is a finite float32.
+MAX_SOFTMAX_SCALE = 2.0e38
+
 _TORCH_DTYPES = {
     torch.float16: DTYPE_F16,
     torch.bfloat16: DTYPE_BF16,

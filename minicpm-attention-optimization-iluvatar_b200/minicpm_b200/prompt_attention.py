@@ -22,7 +22,6 @@ from . import _lib
 
 _INDEX_TYPES = (torch.int32, torch.int64)
 _ELEMENT_TYPES = (torch.bfloat16, torch.float16)
-_MAX_SCALE = 3.0e38
 
 
 def prompt_layout_supported(*rows: torch.Tensor, softmax_scale: float) -> bool:
@@ -38,7 +37,7 @@ def prompt_layout_supported(*rows: torch.Tensor, softmax_scale: float) -> bool:
         st, sh, sd = t.stride()
         if sd != 1 or t.data_ptr() % 16 or (heads > 1 and sh % 8) or (tokens > 1 and st % 8):
             return False
-    return 0.0 < softmax_scale <= _MAX_SCALE
+    return 0.0 < softmax_scale <= _lib.MAX_SOFTMAX_SCALE
 
 
 def prompt_attention(
@@ -94,8 +93,8 @@ def prompt_attention(
         raise ValueError("k and v hold fewer rows than q: pass cu_seqlens_k")
     if max_seqlen_k is None:
         max_seqlen_k = max_seqlen_q if same_k else total_k
-    if not 0.0 < softmax_scale <= _MAX_SCALE:
-        raise ValueError("softmax_scale must be positive and finite")
+    if not 0.0 < softmax_scale <= _lib.MAX_SOFTMAX_SCALE:
+        raise ValueError("softmax_scale must be positive and at most 2e38")
     if not q.is_cuda:
         raise RuntimeError("prompt_attention runs on CUDA tensors only (no CPU path)")
     dtype = q.dtype

@@ -86,8 +86,8 @@ def paged_tree_attention(
     mask_cols = tree_mask.shape[1]
     if mask_cols < max_seqlen_q:
         raise ValueError("tree_mask must have a column for each of the max_seqlen_q drafted tokens")
-    if not 0.0 < softmax_scale <= 3.0e38:
-        raise ValueError("softmax_scale must be positive and finite")
+    if not 0.0 < softmax_scale <= _lib.MAX_SOFTMAX_SCALE:
+        raise ValueError("softmax_scale must be positive and at most 2e38")
     if not q.is_cuda:
         raise RuntimeError("paged_tree_attention runs on CUDA tensors only (no CPU path)")
     dtype = q.dtype
