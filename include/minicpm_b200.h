@@ -546,9 +546,12 @@ B200_API int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable
 B200_API const char* b200_last_error(void);
 
 /*
- * Synchronises `stream`, then reads and clears this library's device error
- * word on the current device (B200_DEVERR_*).  For tests and debugging; the
- * hot-path calls never synchronise.
+ * Synchronises `stream`, then returns and clears a code that this library's
+ * kernels recorded on the current device (B200_DEVERR_*).  Cache writes and paged
+ * attention, prompt attention, tree attention and the page operators record apart,
+ * the first error of each: further ones are returned by the calls that follow,
+ * until one returns B200_DEVERR_NONE.  For tests and debugging; the hot-path calls
+ * never synchronise.
  */
 B200_API int b200_device_error(void* stream, uint32_t* code);
 

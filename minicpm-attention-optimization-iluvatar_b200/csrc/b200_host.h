@@ -25,9 +25,9 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType dt, cuuint32_t rank, const 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
-// The device error word of each translation unit besides b200_lib.cu: read and cleared.
-cudaError_t prompt_device_error(unsigned int* code);
-cudaError_t tree_device_error(unsigned int* code);
-cudaError_t pages_device_error(unsigned int* code);
+// The address of each translation unit's device error word (b200_lib.cu has its own).
+cudaError_t prompt_error_word(void** word);
+cudaError_t tree_error_word(void** word);
+cudaError_t pages_error_word(void** word);
 
 }  // namespace b200_host

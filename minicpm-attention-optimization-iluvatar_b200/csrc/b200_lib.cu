@@ -963,14 +963,18 @@ int b200_device_error(void* stream, uint32_t* code) {
   if (!code) return fail(B200_ERR_INVALID, "null code pointer");
   cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "stream synchronize: %s", cudaGetErrorString(e));
-  unsigned int v = 0, zero = 0;
-  e = cudaMemcpyFromSymbol(&v, b200::g_device_error, sizeof(v));
-  if (e == cudaSuccess) e = cudaMemcpyToSymbol(b200::g_device_error, &zero, sizeof(zero));
-  // Each translation unit has an error word of its own; the first set one is reported, all are cleared.
-  for (auto read : {b200_host::prompt_device_error, b200_host::tree_device_error, b200_host::pages_device_error}) {
-    unsigned int u = 0;
-    if (e == cudaSuccess) e = read(&u);
-    if (v == 0) v = u;
+  // Each translation unit has an error word of its own: the first that is set is
+  // reported and cleared, another one's code waits for the next call.
+  void* words[4] = {};
+  e = cudaGetSymbolAddress(&words[0], b200::g_device_error);
+  if (e == cudaSuccess) e = prompt_error_word(&words[1]);
+  if (e == cudaSuccess) e = tree_error_word(&words[2]);
+  if (e == cudaSuccess) e = pages_error_word(&words[3]);
+  unsigned int v = 0;
+  const unsigned int zero = 0;
+  for (int i = 0; i < 4 && e == cudaSuccess && v == 0; ++i) {
+    e = cudaMemcpy(&v, words[i], sizeof(v), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && v != 0) e = cudaMemcpy(words[i], &zero, sizeof(zero), cudaMemcpyHostToDevice);
   }
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "device error word: %s", cudaGetErrorString(e));
   *code = v;

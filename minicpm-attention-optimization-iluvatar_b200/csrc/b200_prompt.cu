@@ -8,11 +8,7 @@ using namespace b200_host;
 
 namespace b200_host {
 
-cudaError_t prompt_device_error(unsigned int* code) {
-  const unsigned int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(code, b200::g_device_error, sizeof(*code));
-  return e != cudaSuccess ? e : cudaMemcpyToSymbol(b200::g_device_error, &zero, sizeof(zero));
-}
+cudaError_t prompt_error_word(void** word) { return cudaGetSymbolAddress(word, b200::g_device_error); }
 
 }  // namespace b200_host
 

@@ -20,7 +20,7 @@
 
 namespace b200 {
 
-// First device-side error wins; read and cleared by b200_device_error().
+// First device-side error of the translation unit wins; read and cleared by b200_device_error().
 __device__ unsigned int g_device_error = 0;
 
 __device__ __forceinline__ void record_device_error(unsigned int code) {

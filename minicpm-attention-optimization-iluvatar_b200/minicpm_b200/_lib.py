@@ -326,7 +326,11 @@ def varlen_workspace_bytes(device_index: int, *sizes: int) -> int:
 
 
 def device_error(device: torch.device | None = None) -> int:
-    """Synchronise the current stream and return/clear the library's device error word."""
+    """Synchronise the current stream; return and clear a device error code of the library.
+
+    Kernels of different kinds record apart (see ``b200_device_error``): call until it
+    returns ``DEVERR_NONE`` to see every code.
+    """
     lib = load()
     dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
     code = ctypes.c_uint32(0)
