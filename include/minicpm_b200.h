@@ -535,8 +535,8 @@ B200_API int b200_free_sequences(const B200SeqTable* table, const void* rows, in
  * (B200_DEVERR_PAGE_RANGE) or would write a shared page (B200_DEVERR_PAGE_SHARED).
  * A context that is no length (negative, past 2^30 - 1) is recorded as
  * B200_DEVERR_ACCEPT: the row's length becomes 0 and it keeps its pages.
- * seq_lens is written for every row of the table and overlaps neither context_lens
- * nor num_accepted.
+ * seq_lens is written for every row of the table and overlaps none of context_lens,
+ * accepted and num_accepted.
  */
 B200_API int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable* table, const void* context_lens,
                                 const void* accepted, int64_t accepted_stride, int32_t most, const void* num_accepted,

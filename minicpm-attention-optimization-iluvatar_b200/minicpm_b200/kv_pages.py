@@ -223,7 +223,8 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
     ``context_lens[b] + num_accepted[b]``.  ``accepted`` ``[num_seqs, A]`` holds the path's indices
     among the drafted tokens, strictly rising; what is behind ``num_accepted[b]`` is not read.
     With ``ref_counts`` the pages behind the new lengths are released (their table entries
-    become -1) and a shared page is not written to.  A path is cut before its first entry
+    become -1) and a shared page is not written to.  ``seq_lens`` may overlap neither
+    ``context_lens`` nor ``num_accepted``.  A path is cut before its first entry
     that does not rise or has no page of its own, which is recorded; a negative context is
     recorded too, its row keeps its pages and gets length 0.
     """
@@ -246,6 +247,10 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
     stride, step = accepted.stride()
     if most and (step != 1 or stride < most):
         accepted = accepted.contiguous()
+        stride = most
+    begin = accepted.data_ptr()
+    if begin < lens_end and seq_lens.data_ptr() < begin + rows * stride * accepted.element_size():
+        accepted = accepted.clone(memory_format=torch.contiguous_format)  # paths are read while seq_lens is written
         stride = most
     context_lens = context_lens.contiguous()
     lib = _lib.load()
