@@ -30,4 +30,23 @@ cudaError_t prompt_error_word(void** word);
 cudaError_t tree_error_word(void** word);
 cudaError_t pages_error_word(void** word);
 
+// `dependent`: a programmatic dependent of the launch before it, whose end its
+// set-up overlaps; it waits (griddepcontrol.wait) before it reads that kernel's output.
+template <typename... KArgs, typename... Args>
+int launch_form_kernel(const char* what, bool dependent, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem,
+                       cudaStream_t s, const Args&... args) {
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = pdl;
+  cfg.numAttrs = dependent ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+  return check_launch(what);
+}
+
 }  // namespace b200_host

@@ -2,7 +2,7 @@
 //
 // The kernels live in the headers included below; prompt and draft-tree
 // attention and the cache's page operators have translation units of their own
-// (b200_prompt.cu, b200_tree.cu, b200_pages.cu), which compile in parallel.
+// (b200_prompt.cu, b200_tree.cu, b200_join.cu, b200_pages.cu), which compile in parallel.
 // Host code validates arguments (mirroring the reference's ValueError checks
 // in kernels/triton_split_kv_paged.py:249-281 and
 // kernels/triton_rope_kv_cache.py:219-260 where they apply to raw pointers),

@@ -164,7 +164,7 @@ int b200_fork_sequences(const B200PageCaches* caches, const B200SeqTable* table,
   ws += align_up(sizeof(int) * (size_t)a.t.max_seqs, 256);
   a.free_pages = reinterpret_cast<int*>(ws);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  b200::fork_plan_kernel<0><<<1, b200::kForkThreads, 0, s>>>(a);
+  b200::fork_plan_kernel<<<1, b200::kForkThreads, 0, s>>>(a);
   if (int r = check_launch("fork_plan_kernel")) return r;
   const int64_t parts = (a.t.block_size + b200::kForkToks - 1) / b200::kForkToks;
   const dim3 grid = warp_grid(num_entries * std::max<int64_t>(parts, (a.t.cols + 31) / 32), c.shape.num_caches + 1);
@@ -184,7 +184,7 @@ int b200_free_sequences(const B200SeqTable* table, const void* rows, int32_t num
   a.rows = rows;
   a.n = num_rows;
   a.idx_i64 = index_dtype == B200_DTYPE_I64;
-  b200::free_pages_kernel<0><<<num_rows, b200::kPageThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  b200::free_pages_kernel<<<num_rows, b200::kPageThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return check_launch("free_pages_kernel");
 }
 
@@ -223,7 +223,7 @@ int b200_keep_accepted(const B200PageCaches* caches, const B200SeqTable* table, 
   fa.t = a.t;
   fa.n = a.num_seqs;
   fa.context_lens = context_lens;
-  return launch_after("free_pages_kernel", b200::free_pages_kernel<0>, dim3((unsigned)a.num_seqs), s, fa);
+  return launch_after("free_pages_kernel", b200::free_pages_kernel, dim3((unsigned)a.num_seqs), s, fa);
 }
 
 }  // extern "C"

@@ -129,7 +129,6 @@ struct ForkArgs {
 
 // One block: which entries are sound, which need a page, and the lowest free
 // pages for them in the order of the entries.
-template <int kUnused = 0>
 __global__ void __launch_bounds__(kForkThreads, 1) fork_plan_kernel(const ForkArgs a) {
   __shared__ int warp_sums[32];
   griddep_launch_dependents();
@@ -295,7 +294,6 @@ struct FreeArgs {
 
 // One block per row.  An entry is taken out of the table before its page's
 // count goes down, so a row named twice is released once.
-template <int kUnused = 0>
 __global__ void __launch_bounds__(kPageThreads) free_pages_kernel(const FreeArgs a) {
   griddep_wait();
   const int64_t row = a.rows ? load_index64(a.rows, blockIdx.x, a.idx_i64) : static_cast<int64_t>(blockIdx.x);

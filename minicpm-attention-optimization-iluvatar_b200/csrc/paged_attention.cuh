@@ -256,7 +256,7 @@ __device__ __forceinline__ int load_clipped(const void* p, int64_t i, int is_i64
 template <int kForm, typename Args>
 __device__ __forceinline__ SeqBounds seq_bounds(const Args& a, int b) {
   SeqBounds s{};
-  if (kForm == kFormPaged) {
+  if constexpr (kForm == kFormPaged) {
     s.q_begin = load_index(a.cu_q, b, a.len_i64);
     s.q_end = load_index(a.cu_q, b + 1, a.len_i64);
     s.seq_len = load_index(a.seqused, b, a.len_i64);
@@ -264,10 +264,10 @@ __device__ __forceinline__ SeqBounds seq_bounds(const Args& a, int b) {
   }
   s.q_begin = load_clipped(a.cu_q, b, a.len_i64, 0, a.total_q);
   s.q_end = load_clipped(a.cu_q, b + 1, a.len_i64, s.q_begin, a.total_q);
-  if (form_rows(kForm)) {
+  if constexpr (form_rows(kForm)) {
     s.k_begin = load_clipped(a.cu_k, b, a.len_i64, 0, a.total_k);
     s.seq_len = load_clipped(a.cu_k, b + 1, a.len_i64, s.k_begin, a.total_k) - s.k_begin;
-  } else {
+  } else if constexpr (kForm == kFormTree) {
     // A table row holds bt_cols pages; keys past them do not exist.
     const int64_t room = static_cast<int64_t>(a.bt_cols) * a.block_size;
     s.seq_len = load_clipped(a.seqused, b, a.len_i64, 0, min(room, static_cast<int64_t>(0x7fffff00)));
@@ -1574,9 +1574,9 @@ struct SchedArgs {
   int uniform_splits;  // 1: every query unit is split num_splits ways
   int num_sms;
   int capacity;
-  // kFormPrompt / kFormTree: the caller's sizes, which bound what the lengths say.
+  // kFormPrompt: the caller's sizes, which bound what the lengths say.
   const void* cu_k;
-  int total_q, total_k, bt_cols, block_size;
+  int total_q, total_k;
   int max_qunits;    // room in the per-query-unit arrays
   int full;
   int* tile_base;    // [num_seqs + 1]: query units per sequence, exclusive prefix
