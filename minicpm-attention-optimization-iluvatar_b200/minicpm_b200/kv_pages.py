@@ -237,10 +237,12 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
     counts, n, code = _indices("num_accepted", num_accepted, dev)
     if n != rows or counts.dtype != accepted.dtype:
         raise ValueError("num_accepted must hold one count per row, in the dtype of accepted")
-    if abs(context_lens.data_ptr() - seq_lens.data_ptr()) < rows * seq_lens.element_size():
+    # Other sequences' lengths, counts and paths are read while seq_lens is written.
+    lens_begin, lens_bytes = seq_lens.data_ptr(), rows * seq_lens.element_size()
+    index_bytes, counts_begin = counts.element_size(), counts.data_ptr()
+    if abs(context_lens.data_ptr() - lens_begin) < lens_bytes:
         raise ValueError("seq_lens may not be (or overlap) context_lens")
-    lens_end = seq_lens.data_ptr() + rows * seq_lens.element_size()  # other sequences' counts are read while it is written
-    if counts.data_ptr() < lens_end and seq_lens.data_ptr() < counts.data_ptr() + rows * counts.element_size():
+    if counts_begin < lens_begin + lens_bytes and lens_begin < counts_begin + rows * index_bytes:
         raise ValueError("seq_lens may not be (or overlap) num_accepted")
     _on(layers, dev, "keep_accepted_tokens")
     most = accepted.shape[1]
@@ -248,15 +250,15 @@ def keep_accepted_tokens(kv_caches: Caches, block_table: torch.Tensor, context_l
     if most and (step != 1 or stride < most):
         accepted = accepted.contiguous()
         stride = most
-    begin = accepted.data_ptr()
-    if begin < lens_end and seq_lens.data_ptr() < begin + rows * stride * accepted.element_size():
-        accepted = accepted.clone(memory_format=torch.contiguous_format)  # paths are read while seq_lens is written
-        stride = most
+    accepted_begin = accepted.data_ptr()
+    if accepted_begin < lens_begin + lens_bytes and lens_begin < accepted_begin + rows * stride * index_bytes:
+        accepted = accepted.clone(memory_format=torch.contiguous_format)
+        accepted_begin, stride = accepted.data_ptr(), most
     context_lens = context_lens.contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
-        _lib.check(lib.b200_keep_accepted(layers._ref, ctypes.byref(table), context_lens.data_ptr(), accepted.data_ptr(),
-                                          max(stride, most), most, counts.data_ptr(), code, _lib.current_stream(dev)),
+        _lib.check(lib.b200_keep_accepted(layers._ref, ctypes.byref(table), context_lens.data_ptr(), accepted_begin,
+                                          max(stride, most), most, counts_begin, code, _lib.current_stream(dev)),
                    "keep_accepted_tokens")
 
 
