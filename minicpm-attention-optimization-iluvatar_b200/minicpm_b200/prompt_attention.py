@@ -3,10 +3,11 @@
 The first pass over a prompt, an encoder batch or an embedding batch needs no
 cache: sequences of different lengths lie one after the other in ``q``, ``k`` and
 ``v`` (``cu_seqlens``), query heads share KV heads (any ratio up to 128) and a row
-sees its sequence causally or whole.  One call of ``b200_prompt_attn_fwd``: a
-device-side work list, the tcgen05 attention kernel in its form for plain rows
-and, for batches too small to fill the GPU, a combine of split keys, all on the
-current CUDA stream without a host synchronisation.  No counterpart in the
+sees its sequence causally or whole.  One call of ``b200_prompt_attn_fwd``: for
+batches that fill the GPU a device-side work list and the tcgen05 attention kernel in
+its form for plain rows; else that kernel alone, whose CTAs divide all keys among
+themselves, and a join of the units that several of them share.  All on the current
+CUDA stream without a host synchronisation.  No counterpart in the
 reference, whose service sends encoder batches to vLLM
 (``integration/vllm-plugin-FL-split-kv.patch:785-813``).
 """
@@ -64,8 +65,8 @@ def prompt_attention(
     sequence are left as they were, and rows of ``k``/``v`` that belong to none may
     hold anything; the keys and values of a sequence must be finite.
 
-    ``max_seqlen_k`` (None: ``max_seqlen_q``) is the longest key sequence; it only
-    bounds how far keys are split.  The scores, the softmax statistics and the output
+    ``max_seqlen_k`` is the longest key sequence (None: ``max_seqlen_q``, or all keys
+    where ``cu_seqlens_k`` is given); it only bounds how far keys are split.  The scores, the softmax statistics and the output
     are held in fp32; the softmax weights are rounded to the element type for the
     second product.
     """

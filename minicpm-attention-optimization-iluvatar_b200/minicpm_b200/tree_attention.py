@@ -3,9 +3,9 @@
 Speculative decoding verifies the drafted tokens of every sequence in one pass:
 their K/V rows are written to the cache behind the context (as any new token's),
 and each token attends to the context and to its own ancestors in the tree.  One
-call of ``b200_tree_attn_fwd``: a device-side work list, the tcgen05 attention kernel
-in its form for trees, and a combine of split keys, on the current CUDA stream
-without a host synchronisation.  No counterpart in the reference.
+call of ``b200_tree_attn_fwd``: the tcgen05 attention kernel in its form for trees, whose
+CTAs divide all keys among themselves, and a join of the units that several of them
+share, on the current CUDA stream without a host synchronisation.  No counterpart in the reference.
 :func:`minicpm_b200.kv_pages.keep_accepted_tokens` then moves the accepted path
 together in the cache.
 """
